@@ -333,6 +333,82 @@ int hqm_rope_append_rows(uint16_t* q, const uint16_t* k, const uint16_t* v, uint
                          int64_t batch_stride, const int64_t* pos_device, int32_t pos0, int32_t pos_step, float rope_theta,
                          void* stream);
 
+/* ---- a key/value cache in pages -------------------------------------------- */
+/* No counterpart in the reference, whose Hugging Face cache is one tensor per layer (build_model.py:166-241 hands
+ * generation to Hugging Face).  Sequences of different lengths share one pool of pages: a layer's keys (and its values) are
+ * (pages, n_kv_heads, page_size, head_dim), page_size a power of two; sequence b holds its first kv_lens[b] positions in
+ * the pages block_table[b][0 ..].  The pages that nobody holds are the stack free_pages[0 .. *free_count - 1]
+ * (`capacity` entries).  All of it is int32 in device memory, so nothing returns to the host.
+ *
+ * hqm_paged_reserve: new_lens[b] more positions for every sequence.  Takes pages off the top of the stack, in the order of
+ * the sequences, writes them into block_table, adds to kv_lens, and writes, for the step that follows, cu_seqlens (sequences
+ * + 1): the first row of every sequence among its tokens; kv_lens_after (sequences): the lengths with the new tokens;
+ * positions and slots (tokens): position of every new token, and page * page_size + row of its place (-1 behind the last
+ * token).  All or nothing: *status is 0, or the number of missing pages, or -1: a negative length, or one that no row of
+ * max_pages holds, -2: more new tokens than `tokens`, -3: *free_count is not 0 .. capacity; then lengths, tables and
+ * stack stay, cu_seqlens is all 0 (the step has no tokens) and every position and slot -1.  At most 16384 sequences. */
+int hqm_paged_reserve(int32_t* block_table, int64_t table_stride, int32_t* kv_lens, const int32_t* free_pages, int32_t* free_count,
+                      const int32_t* new_lens, int32_t* cu_seqlens, int32_t* kv_lens_after, int32_t* positions, int32_t* slots,
+                      int32_t* status, int32_t sequences, int32_t max_pages, int32_t page_size, int32_t capacity, int64_t tokens,
+                      void* stream);
+/* Every sequence keeps its first keep[b] positions (0: it has ended; fewer than before: rejected tokens); the pages behind
+ * go back on the stack, in the order in which hqm_paged_reserve would hand them out again.  *status is 0, -1: keep[b] is
+ * negative or beyond the length, -3: the stack would not hold them (a page given back twice); then nothing changes. */
+int hqm_paged_truncate(const int32_t* block_table, int64_t table_stride, int32_t* kv_lens, int32_t* free_pages, int32_t* free_count,
+                       const int32_t* keep, int32_t* status, int32_t sequences, int32_t max_pages, int32_t page_size, int32_t capacity,
+                       void* stream);
+
+/* Rotary embedding (rotate-half) of q and k at every token's position, and the append of k and v at its slot.  Unlike
+ * hqm_rope_append_rows, which rounds to bf16 after every operation as Hugging Face does, angles are formed in 64 bits and a
+ * result is rounded once.  q (tokens, n_heads, head_dim), k and v (tokens, n_kv_heads, head_dim), strides in elements,
+ * multiples of 8, rows 16-byte aligned; q_out (tokens, n_heads, head_dim) contiguous, may be q.  A token whose slot is
+ * negative is left out (its row of q_out stays); one beyond the pool is too, and makes hqm_device_error() return 2. */
+typedef struct hqm_paged_append {
+    void* q_out;
+    const void *q, *k, *v;
+    int64_t q_token, q_head, k_token, k_head, v_token, v_head;
+    void *k_pages, *v_pages;
+    int64_t k_page, v_page;             /* elements from page to page */
+    const int32_t *positions, *slots;
+    int64_t tokens;
+    int32_t n_heads, n_kv_heads, head_dim, pages, page_size;
+    int32_t dtype;                      /* 0 bf16, 1 fp16 */
+    float rope_theta;
+    int32_t reserved;
+} hqm_paged_append;
+int hqm_rope_append_paged(const hqm_paged_append* a, void* stream);
+
+/* out = softmax(scale * q k^T) v for the new tokens of many sequences at once: sequence b's are rows cu_seqlens[b] ..
+ * cu_seqlens[b + 1] - 1 of q (tokens, n_heads, head_dim) and of out (contiguous).  With n of them and L positions in all, new
+ * token i sees positions 0 .. L - n + i; n_heads / n_kv_heads query heads share a key/value head.  A row that sees nothing
+ * (L - n + i < 0) is 0; rows behind the last sequence are left as they were.  Maximum, total and sums are fp32, the weights
+ * are rounded to dtype for the product with v.  What pages hold behind a sequence may be anything, NaN included; inside a
+ * sequence a value that is not finite may reach every row of the sequence.
+ *   hqm_paged_attention: k and v are pages, L = kv_lens[b] (the new tokens' keys and values are in the pages already);
+ *     page_size 16 or more.  An entry of block_table outside the pool reads as zeros.
+ *   hqm_prompt_attention: k and v (tokens, n_kv_heads, head_dim) lie like q, L = n; block_table, kv_lens and what describes
+ *     pages are not used.
+ * max_new: no sequence has more new tokens than this.  Nothing about lengths is read on the host, so a captured call follows
+ * them.  head_dim 64 or 128; strides in elements, multiples of 8, rows 16-byte aligned.  scratch: any 16-byte aligned memory
+ * of hqm_attention_scratch_bytes bytes that no other call in flight uses (nothing in it has to be initialised). */
+typedef struct hqm_attention {
+    void* out;
+    const void *q, *k, *v;
+    int64_t q_token, q_head, k_token, k_head, v_token, v_head;
+    int64_t k_page, v_page;             /* elements from page to page */
+    const int32_t* block_table;
+    int64_t table_stride;
+    const int32_t *cu_seqlens, *kv_lens;
+    int64_t tokens;
+    int32_t sequences, max_new;
+    int32_t n_heads, n_kv_heads, head_dim, pages, page_size, max_pages;
+    int32_t dtype;                      /* 0 bf16, 1 fp16 */
+    float scale;
+} hqm_attention;
+size_t hqm_attention_scratch_bytes(const hqm_attention* call);
+int hqm_paged_attention(const hqm_attention* call, void* scratch, size_t scratch_bytes, void* stream);
+int hqm_prompt_attention(const hqm_attention* call, void* scratch, size_t scratch_bytes, void* stream);
+
 /* ---- expert residency: src/expert_cache.py -------------------------------- */
 /* ExpertCache (expert_cache.py:55-201).  The handle owns the bookkeeping of
  * ExpertInfo / EvictionGroupInfo (expert_cache.py:12-52), a side copy stream and

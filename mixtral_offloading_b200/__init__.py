@@ -11,5 +11,7 @@ from .decoder import (AttentionDecode, DecoderLayerDecode, ExpertParallelDecoder
                       add_rmsnorm)
 from .expert_cache import ExpertCache  # noqa: F401
 from .offload_model import MixtralOffloadModel  # noqa: F401
+from .paged import (PagedStep, paged_attention, paged_reserve, paged_truncate, prompt_attention,  # noqa: F401
+                    rope_append_paged)
 from .expert_wrapper import MixtralExpertWrapper  # noqa: F401
 from .quantize import BaseQuantizeConfig  # noqa: F401

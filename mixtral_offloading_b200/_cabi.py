@@ -53,6 +53,32 @@ class HqmEpComm(C.Structure):
     ]
 
 
+class HqmPagedAppend(C.Structure):
+    """struct hqm_paged_append."""
+    _fields_ = [
+        ("q_out", C.c_void_p), ("q", C.c_void_p), ("k", C.c_void_p), ("v", C.c_void_p),
+        ("q_token", C.c_int64), ("q_head", C.c_int64), ("k_token", C.c_int64), ("k_head", C.c_int64),
+        ("v_token", C.c_int64), ("v_head", C.c_int64), ("k_pages", C.c_void_p), ("v_pages", C.c_void_p),
+        ("k_page", C.c_int64), ("v_page", C.c_int64), ("positions", C.c_void_p), ("slots", C.c_void_p),
+        ("tokens", C.c_int64), ("n_heads", C.c_int32), ("n_kv_heads", C.c_int32), ("head_dim", C.c_int32),
+        ("pages", C.c_int32), ("page_size", C.c_int32), ("dtype", C.c_int32), ("rope_theta", C.c_float),
+        ("reserved", C.c_int32),
+    ]
+
+
+class HqmAttention(C.Structure):
+    """struct hqm_attention."""
+    _fields_ = [
+        ("out", C.c_void_p), ("q", C.c_void_p), ("k", C.c_void_p), ("v", C.c_void_p),
+        ("q_token", C.c_int64), ("q_head", C.c_int64), ("k_token", C.c_int64), ("k_head", C.c_int64),
+        ("v_token", C.c_int64), ("v_head", C.c_int64), ("k_page", C.c_int64), ("v_page", C.c_int64),
+        ("block_table", C.c_void_p), ("table_stride", C.c_int64), ("cu_seqlens", C.c_void_p), ("kv_lens", C.c_void_p),
+        ("tokens", C.c_int64), ("sequences", C.c_int32), ("max_new", C.c_int32), ("n_heads", C.c_int32),
+        ("n_kv_heads", C.c_int32), ("head_dim", C.c_int32), ("pages", C.c_int32), ("page_size", C.c_int32),
+        ("max_pages", C.c_int32), ("dtype", C.c_int32), ("scale", C.c_float),
+    ]
+
+
 _P = C.c_void_p
 _I64 = C.c_int64
 _I32 = C.c_int32
@@ -108,6 +134,12 @@ SIGNATURES = {
     "hqm_add_rmsnorm_rows": (C.c_int, [_P, _P, _P, _P, C.c_int64, _I32, C.c_float, _P]),
     "hqm_rope_append_rows": (C.c_int, [_P, _P, _P, _P, _P, C.c_int64, _I32, _I32, _I32, _I32, C.c_int64, _P, _I32, _I32,
                                        C.c_float, _P]),
+    "hqm_paged_reserve": (C.c_int, [_P, _I64, _P, _P, _P, _P, _P, _P, _P, _P, _P, _I32, _I32, _I32, _I32, _I64, _P]),
+    "hqm_paged_truncate": (C.c_int, [_P, _I64, _P, _P, _P, _P, _P, _I32, _I32, _I32, _I32, _P]),
+    "hqm_rope_append_paged": (C.c_int, [C.POINTER(HqmPagedAppend), _P]),
+    "hqm_attention_scratch_bytes": (C.c_size_t, [C.POINTER(HqmAttention)]),
+    "hqm_paged_attention": (C.c_int, [C.POINTER(HqmAttention), _P, C.c_size_t, _P]),
+    "hqm_prompt_attention": (C.c_int, [C.POINTER(HqmAttention), _P, C.c_size_t, _P]),
     "hqm_router_top2": (C.c_int, [_P, _P, _P, _P, _P, _P, _P, _P, _P, _I64, _I64, _I32, _P]),
     "hqm_cache_create": (C.c_int, [C.POINTER(_P), _I32, _I32, _I32, C.c_size_t, C.POINTER(_P), _I32]),
     "hqm_cache_destroy": (None, [_P]),

@@ -1,0 +1,231 @@
+// What the attention kernels over new tokens share: their arguments, how the work is cut, and the partial results.
+//
+// A launch covers sequences of different lengths: sequence b has n_b new tokens (rows cu[b] .. cu[b + 1] of q) and L_b
+// positions of keys and values, the new ones last; new token i sees positions 0 .. L_b - n_b + i.  The `group` query heads of one
+// key/value head are rows of the same tile (row = token * group + head), so that keys and values are read once for all of them.
+//
+// The work is a list of units (sequence, key/value head, tile of rows), each of as many blocks of keys as its last row sees, at
+// least one.  The list's blocks are cut into equal runs, one per CTA, wherever that falls: every CTA finds its run from the
+// lengths in device memory, so the host needs no length and a captured graph follows them.  A unit that a cut goes through leaves
+// unnormalised sums with their maximum and total (a "piece") per CTA, which attn_join adds in the order of the CTAs: the same
+// bits for the same lengths, whichever CTA ends first.
+#pragma once
+#include <cuda.h>
+
+#include "common.cuh"
+#include "kernels.cuh"
+
+namespace hqm {
+namespace attn {
+
+struct Args {
+    const uint16_t* q;
+    uint16_t* out;                 // (T, n_heads, D), contiguous
+    int64_t q_token, q_head;       // strides of q, in elements
+    const int32_t* table;          // null: keys and values are packed like the queries
+    int64_t table_stride;
+    const int32_t* cu;             // B + 1
+    const int32_t* kv_lens;        // null with table
+    int B, T, n_kv, group;
+    int n_pages, max_pages, page_shift;
+    float scale_log2;              // softmax scale times log2(e)
+    float* pieces;                 // two per CTA
+    int32_t* records;              // of CTA c: the unit that starts in c and is cut behind it (RECORD words)
+    int piece_rows;                // rows of a piece
+};
+constexpr int RECORD = 8;          // q0, tokens, head, first token, CTAs (0: none), 3 unused
+
+// Sum of floor((a i + b) / m) over i = 0 .. n - 1, for a, b >= 0 (the sum of an arithmetic progression per step of Euclid's algorithm on a, m).
+__host__ __device__ inline int64_t floor_sum(int64_t n, int64_t m, int64_t a, int64_t b) {
+    int64_t sum = 0;
+    while (n > 0) {
+        if (a >= m) { sum += (n - 1) * n / 2 * (a / m); a %= m; }
+        if (b >= m) { sum += n * (b / m); b %= m; }
+        const int64_t y = a * n + b;
+        if (y < m) break;
+        n = y / m;
+        b = y % m;
+        const int64_t t = m;
+        m = a;
+        a = t;
+    }
+    return sum;
+}
+
+// One sequence's part of the list.
+struct Seq {
+    int q0, n;                     // rows of q
+    int kv;                        // positions that can be read
+    int before;                    // kv - n: what token 0 sees, less one
+    int tiles, per;                // tiles of rows, tokens per tile
+    int block;                     // keys per block
+    __host__ __device__ int blocks(int tile) const {
+        const int seen = before + min((tile + 1) * per, n);
+        return max(1, (seen + block - 1) / block);
+    }
+    // blocks of tiles 0 .. count - 1
+    __host__ __device__ int64_t prefix(int count) const {
+        const int whole = min(count, tiles - 1);               // tiles of `per` tokens
+        int empty = 0;                                         // of them, the ones that see nothing: one block each
+        if (before < 0) empty = min(whole, (-before) / per);
+        int64_t sum = empty + floor_sum(whole - empty, block, per, (int64_t)before + (int64_t)(empty + 1) * per + block - 1);
+        if (count >= tiles && tiles > 0) sum += blocks(tiles - 1);
+        return sum;
+    }
+    __host__ __device__ int64_t total() const { return prefix(tiles); }
+};
+
+__device__ __forceinline__ Seq load_seq(const Args& a, int b, int per, int block) {
+    Seq s;
+    const int lo = min(max(a.cu[b], 0), a.T), hi = min(max(a.cu[b + 1], lo), a.T);
+    s.q0 = lo;
+    s.n = hi - lo;
+    s.kv = s.n;
+    if (a.table) s.kv = (int)min((int64_t)max(a.kv_lens[b], 0), (int64_t)a.max_pages << a.page_shift);
+    s.before = s.kv - s.n;
+    s.per = per;
+    s.block = block;
+    s.tiles = (s.n + per - 1) / per;
+    return s;
+}
+
+// Where a CTA's run of blocks begins, and how long it is.
+struct Run {
+    int64_t share;                 // blocks of every run (the last one may have fewer)
+    int64_t left;                  // blocks of this one
+    int b, h, tile;
+    int skip;                      // blocks of its first unit that belong to earlier CTAs
+};
+
+// Called by one whole warp; every lane gets the run.
+__device__ inline Run find_run(const Args& a, int per, int block) {
+    const int lane = threadIdx.x & 31;
+    int64_t total = 0;
+    for (int b0 = 0; b0 < a.B; b0 += 32) {
+        int64_t w = 0;
+        if (b0 + lane < a.B) w = load_seq(a, b0 + lane, per, block).total() * a.n_kv;
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) w += __shfl_xor_sync(0xffffffffu, w, o);
+        total += w;
+    }
+    Run r;
+    r.share = (total + gridDim.x - 1) / gridDim.x;
+    const int64_t lo = r.share * blockIdx.x;
+    r.left = min(max(total - lo, (int64_t)0), r.share);
+    r.b = r.h = r.tile = r.skip = 0;
+    if (r.left == 0) return r;
+    int64_t base = 0;
+    for (int b0 = 0; b0 < a.B; b0 += 32) {
+        int64_t w = 0;
+        if (b0 + lane < a.B) w = load_seq(a, b0 + lane, per, block).total() * a.n_kv;
+        int64_t sum = w;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int64_t v = __shfl_up_sync(0xffffffffu, sum, o);
+            if (lane >= o) sum += v;
+        }
+        const uint32_t past = __ballot_sync(0xffffffffu, base + sum > lo);
+        if (past) {
+            const int src = __ffs(past) - 1;
+            r.b = b0 + src;
+            const int64_t off = lo - (base + __shfl_sync(0xffffffffu, sum - w, src));
+            const Seq s = load_seq(a, r.b, per, block);
+            const int64_t one = s.total();
+            r.h = (int)(off / one);
+            const int64_t in = off - r.h * one;
+            int t0 = 0, t1 = s.tiles - 1;                      // the last tile whose prefix is <= in
+            while (t0 < t1) {
+                const int mid = (t0 + t1 + 1) / 2;
+                if (s.prefix(mid) <= in) t0 = mid;
+                else t1 = mid - 1;
+            }
+            r.tile = t0;
+            r.skip = (int)(in - s.prefix(t0));
+            return r;
+        }
+        base += __shfl_sync(0xffffffffu, sum, 31);
+    }
+    r.left = 0;
+    return r;
+}
+
+// A CTA's walk through its run: every part of a unit that it works on, in order.  All threads that walk it see the same.
+struct Walk {
+    const Args& a;
+    Seq s;
+    int64_t left;
+    int b, h, tile, skip;
+    int j0, j1, blocks;            // the part: blocks j0 .. j1 - 1 of `blocks`
+    __device__ Walk(const Args& args, const Run& r, int per, int block) : a(args), left(r.left), b(r.b), h(r.h), tile(r.tile), skip(r.skip) {
+        if (left > 0) s = load_seq(a, b, per, block);
+    }
+    __device__ bool next() {       // false: done
+        if (left <= 0) return false;
+        if (tile == s.tiles) {
+            tile = 0;
+            if (++h == a.n_kv) {
+                h = 0;
+                do s = load_seq(a, ++b, s.per, s.block);
+                while (s.tiles == 0);
+            }
+        }
+        blocks = s.blocks(tile);
+        j0 = skip;
+        j1 = (int)min((int64_t)blocks, j0 + left);
+        left -= j1 - j0;
+        skip = 0;
+        ++tile;
+        return true;
+    }
+    // the part's tile is tile - 1 from here on
+    __device__ int first_token() const { return (tile - 1) * s.per; }
+    __device__ int tokens() const { return min(s.per, s.n - first_token()); }
+    __device__ bool whole() const { return j0 == 0 && j1 == blocks; }
+};
+
+// A piece: sums [rows][D], then maxima [rows] (base 2), then totals [rows].
+template <int D>
+__device__ __forceinline__ float* piece_at(const Args& a, int cta, int tail) {
+    return a.pieces + (int64_t)(2 * cta + tail) * a.piece_rows * (D + 2);
+}
+inline size_t piece_bytes(int ctas, int rows, int D) { return (size_t)2 * ctas * rows * (D + 2) * sizeof(float); }
+inline size_t record_bytes(int ctas) { return ((size_t)ctas * RECORD * sizeof(int32_t) + 255) / 256 * 256; }
+
+// CTA c's record: about the unit that its run ends in the middle of and that began in it, if there is one.
+__device__ __forceinline__ void write_record(const Args& a, const Walk* w, int64_t share) {
+    int32_t* r = a.records + (int64_t)blockIdx.x * RECORD;
+    if (!w) {
+        r[4] = 0;
+        return;
+    }
+    r[0] = w->s.q0;
+    r[1] = w->tokens();
+    r[2] = w->h;
+    r[3] = w->first_token();
+    r[4] = 1 + (int)((w->blocks - w->j1 + share - 1) / share);      // this CTA and those that the rest reaches into
+}
+
+__device__ __forceinline__ uint16_t to_bits(float v, bool f16) {
+    return f16 ? __half_as_ushort(__float2half_rn(v)) : float_to_bf16_bits(v);
+}
+__device__ __forceinline__ uint32_t pack2(float lo, float hi, bool f16) {      // lo in the lower half
+    uint32_t r;
+    if (f16) asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+    else asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+    return r;
+}
+__device__ __forceinline__ float ex2(float x) {
+    float r;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+    return r;
+}
+
+// Adds the pieces of the units that a cut goes through (attn_few.cu).
+int launch_join(const Args& a, int ctas, int D, bool f16, cudaStream_t st);
+int launch_few(const Args& a, const CUtensorMap& km, const CUtensorMap& vm, int ctas, int D, bool f16, cudaStream_t st);
+
+constexpr int FEW_TILE = 16;       // rows of a tile of attn_few.cu
+constexpr int FEW_KEYS = 64;
+
+}  // namespace attn
+}  // namespace hqm
