@@ -23,11 +23,11 @@ int sm_count() {
     return n;
 }
 
-// Boxes of `rows` x 64 elements, 128-byte swizzle; strides in elements.
-bool encode(CUtensorMap* to, const void* at, const cuuint64_t (&dims)[4], const int64_t (&strides)[3], int rows, int heads, bool f16) {
+// Boxes of 64 x y x z x w elements, 128-byte swizzle; strides in elements.
+bool encode(CUtensorMap* to, const void* at, const cuuint64_t (&dims)[4], const int64_t (&strides)[3], int y, int z, int w, bool f16) {
     const EncodeTiledFn enc = (EncodeTiledFn)tma_encode_entry();
     if (!enc) return false;
-    const cuuint32_t ones[4] = {1, 1, 1, 1}, box[4] = {64, (cuuint32_t)rows, (cuuint32_t)heads, 1};
+    const cuuint32_t ones[4] = {1, 1, 1, 1}, box[4] = {64, (cuuint32_t)y, (cuuint32_t)z, (cuuint32_t)w};
     const cuuint64_t bytes[3] = {(cuuint64_t)strides[0] * 2, (cuuint64_t)strides[1] * 2, (cuuint64_t)strides[2] * 2};
     return enc(to, f16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, const_cast<void*>(at), dims, bytes, box, ones,
                CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
@@ -42,9 +42,9 @@ int check(const hqm_attention* c, bool paged, const char* what) {
                   what, (long long)c->tokens, c->sequences, c->max_new);
     HQM_CHECK_ARG((c->head_dim == 64 || c->head_dim == 128) && (c->dtype == 0 || c->dtype == 1), "%s: head_dim %d (64 or 128), dtype %d (0 bf16, 1 fp16)",
                   what, c->head_dim, c->dtype);
-    HQM_CHECK_ARG(c->n_kv_heads > 0 && c->n_heads > 0 && c->n_heads % c->n_kv_heads == 0 && c->n_heads / c->n_kv_heads <= FEW_TILE,
-                  "%s: %d query heads on %d key/value heads (a multiple, at most %d times)", what, c->n_heads, c->n_kv_heads, FEW_TILE);
-    HQM_CHECK_ARG(isfinite(c->scale), "%s: scale %g", what, (double)c->scale);
+    HQM_CHECK_ARG(c->n_kv_heads > 0 && c->n_heads > 0 && c->n_heads % c->n_kv_heads == 0 && c->n_heads / c->n_kv_heads <= MAX_GROUP,
+                  "%s: %d query heads on %d key/value heads (a multiple, at most %d times)", what, c->n_heads, c->n_kv_heads, MAX_GROUP);
+    HQM_CHECK_ARG(c->scale > 0.f && isfinite(c->scale), "%s: scale %g (positive)", what, (double)c->scale);
     if (paged) {
         const int64_t page_elements = (int64_t)c->n_kv_heads * c->page_size * c->head_dim;
         HQM_CHECK_ARG(c->page_size >= 16 && (c->page_size & (c->page_size - 1)) == 0 && c->pages > 0 && c->max_pages > 0 &&
@@ -63,7 +63,9 @@ int check(const hqm_attention* c, bool paged, const char* what) {
     return HQM_OK;
 }
 
-int rows_of_piece(const hqm_attention* c) { return FEW_TILE; }
+// Whether a unit of attn_few.cu holds all new tokens of any sequence.
+bool few_rows(const hqm_attention* c) { return (int64_t)c->max_new * (c->n_heads / c->n_kv_heads) <= FEW_TILE; }
+int rows_of_piece(const hqm_attention* c) { return few_rows(c) ? FEW_TILE : 2 * TILE_KEYS; }
 
 int run(const hqm_attention* c, bool paged, const char* what, void* scratch, size_t scratch_bytes, void* stream) {
     if (int rc = check(c, paged, what)) return rc;
@@ -99,23 +101,29 @@ int run(const hqm_attention* c, bool paged, const char* what, void* scratch, siz
     a.records = (int32_t*)scratch;
     a.pieces = (float*)((uint8_t*)scratch + record_bytes(ctas));
     a.piece_rows = rows_of_piece(c);
-    CUtensorMap km, vm;
-    const int box = paged && c->page_size < FEW_KEYS ? c->page_size : FEW_KEYS;
+    CUtensorMap qm, km, vm;
+    const bool few = few_rows(c);
+    const int keys = few ? FEW_KEYS : TILE_KEYS, box = paged && c->page_size < keys ? c->page_size : keys;
     bool ok;
     if (paged) {
         const cuuint64_t dims[4] = {(cuuint64_t)D, (cuuint64_t)c->page_size, (cuuint64_t)c->n_kv_heads, (cuuint64_t)c->pages};
         const int64_t head = (int64_t)c->page_size * D;
-        ok = encode(&km, c->k, dims, {(int64_t)D, head, c->k_page}, box, 1, f16) && encode(&vm, c->v, dims, {(int64_t)D, head, c->v_page}, box, 1, f16);
+        ok = encode(&km, c->k, dims, {(int64_t)D, head, c->k_page}, box, 1, 1, f16) && encode(&vm, c->v, dims, {(int64_t)D, head, c->v_page}, box, 1, 1, f16);
     } else {
         const cuuint64_t dims[4] = {(cuuint64_t)D, (cuuint64_t)c->tokens, (cuuint64_t)c->n_kv_heads, 1};
-        ok = encode(&km, c->k, dims, {c->k_token, c->k_head, c->k_token * c->tokens}, box, 1, f16) && encode(&vm, c->v, dims, {c->v_token, c->v_head, c->v_token * c->tokens}, box, 1, f16);
+        ok = encode(&km, c->k, dims, {c->k_token, c->k_head, c->k_token * c->tokens}, box, 1, 1, f16) && encode(&vm, c->v, dims, {c->v_token, c->v_head, c->v_token * c->tokens}, box, 1, 1, f16);
+    }
+    if (ok && !few) {
+        // row = token * group + head: a box of all heads of a group and as many tokens as a tile holds
+        const cuuint64_t dims[4] = {(cuuint64_t)D, (cuuint64_t)a.group, (cuuint64_t)c->n_kv_heads, (cuuint64_t)c->tokens};
+        ok = encode(&qm, c->q, dims, {c->q_head, c->q_head * a.group, c->q_token}, a.group, 1, 128 / a.group, f16);
     }
     if (!ok) {
         set_error("%s: the driver does not encode the tensor maps", what);
         return HQM_ERR_CUDA;
     }
     const cudaStream_t st = (cudaStream_t)stream;
-    if (int rc = launch_few(a, km, vm, ctas, D, f16, st)) return rc;
+    if (int rc = few ? launch_few(a, km, vm, ctas, D, f16, st) : launch_tiles(a, qm, km, vm, ctas, D, f16, st)) return rc;
     return launch_join(a, ctas, D, f16, st);
 }
 

@@ -222,10 +222,16 @@ __device__ __forceinline__ float ex2(float x) {
 
 // Adds the pieces of the units that a cut goes through (attn_few.cu).
 int launch_join(const Args& a, int ctas, int D, bool f16, cudaStream_t st);
+// attn_few.cu: up to FEW_TILE rows per key/value head.
 int launch_few(const Args& a, const CUtensorMap& km, const CUtensorMap& vm, int ctas, int D, bool f16, cudaStream_t st);
 
-constexpr int FEW_TILE = 16;       // rows of a tile of attn_few.cu
-constexpr int FEW_KEYS = 64;
+// attn_tiles.cu: any number.
+int launch_tiles(const Args& a, const CUtensorMap& qm, const CUtensorMap& km, const CUtensorMap& vm, int ctas, int D, bool f16, cudaStream_t st);
+
+constexpr int FEW_TILE = 16;       // rows of a unit of attn_few.cu
+constexpr int FEW_KEYS = 64;       // positions of a block there
+constexpr int TILE_KEYS = 128;     // and in attn_tiles.cu
+constexpr int MAX_GROUP = 128;     // query heads per key/value head: the rows of a tile
 
 }  // namespace attn
 }  // namespace hqm

@@ -1,0 +1,469 @@
+// Attention of many rows per key/value head: prompts, chunks of new tokens, and single tokens beside them, on the
+// 5th-generation tensor cores.
+//
+//     S = Q K^T;  p = 2^(S scale log2 e - m);  O = p V;  l = sum p;  out = O / l
+//
+// One CTA per SM works through its run of the list of units (attn.cuh).  A unit is 256 rows, two tiles of 128 (row = token *
+// group + head), over blocks of 128 positions.  Per block and tile two matrix products of 128 x 128 x D are issued, S into
+// tensor memory, and O from p (in tensor memory, over the S that it came from) and V.  A thread of the four warps of a tile
+// owns one row: maximum, total and weights of a row need no other thread.  While one tile's warps form weights the tensor
+// cores work on the other tile's products.
+//
+// Warps 0-3: weights of tile 0, 4-7: of tile 1, 8: issues the products, 9: copies (cp.async.bulk.tensor; Q once per unit, K and
+// V of every block through a ring of five buffers, of a paged cache a copy per page); 10: walks the list of units; 11
+// only completes the warpgroup.
+//
+// The maximum m that a row's weights refer to is raised only when a block exceeds it by more than 2^8: O, which lies in tensor
+// memory, is rescaled a few times per unit instead of once per block, weights grow to 256 at the most, and l and O mean the same
+// whatever m is.
+#include "attn.cuh"
+#include "shared_limit.h"
+#include "tc_common.cuh"
+
+namespace hqm {
+namespace attn {
+namespace {
+
+constexpr int KEYS = TILE_KEYS;
+constexpr int RING = 5;
+// Three warpgroups of 168 registers a thread at the launch (64512): the two that form weights take 216, the third keeps 72.
+constexpr int THREADS = 384;
+constexpr int REGS_WEIGHTS = 216, REGS_OTHERS = 72;
+static_assert(256 * REGS_WEIGHTS + 128 * REGS_OTHERS <= THREADS * 168, "registers of the launch");
+constexpr float SLACK = 8.f;
+
+// A part of a unit (Walk), as the warp that walks the list hands it to the others.
+struct Part {
+    int tokens;                    // 0: the end of the list
+    int q_row, head;               // row of q and out of the first token
+    int sees, kv;                  // positions that the first token sees, positions of the sequence
+    int j0, j1;                    // blocks
+    int kv_row, table_row;         // where the sequence begins: packed keys, pages
+    int whole;                     // 1: no cut goes through the unit; else 2: its first piece, 0: a later one
+};
+constexpr int PARTS = 4;
+
+template <int D>
+struct Shared {
+    static constexpr int HALVES = D / 64;
+    static constexpr int PANEL = 128 * 128;                       // 128 rows x 64 columns, 128-byte swizzle
+    static constexpr int TILE = HALVES * PANEL;
+    alignas(1024) unsigned char q[2][TILE];
+    alignas(1024) unsigned char ring[RING][TILE];                 // K, V, K, V, ...
+    uint64_t full[RING], empty[RING], q_full, q_empty, s_full[2], p_full[2], o_done[2];
+    uint64_t part_full[PARTS], part_empty[PARTS];
+    Part parts[PARTS];                                            // tokens = 0: the end
+    uint32_t tmem;
+};
+
+// Waits until the phase of this parity is over; false (at once from then on) when it has taken about a second.
+struct Patience {
+    bool ok = true;
+    __device__ __forceinline__ void wait(uint64_t* bar, uint32_t parity) {
+        const uint32_t at = tc::smem_u32(bar);
+        uint32_t done = !ok;
+        long long began = 0;
+        while (!done) {
+            asm volatile(
+                "{\n\t.reg .pred p;\n\t"
+                "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+                "selp.u32 %0, 1, 0, p;\n\t}"
+                : "=r"(done) : "r"(at), "r"(parity) : "memory");
+            if (!done) {
+                const long long now = clock64();
+                if (began == 0) began = now;
+                else if (now - began > 2000000000ll) { ok = false; return; }
+            }
+        }
+    }
+};
+
+__device__ __forceinline__ void expect(uint64_t* bar, uint32_t bytes) {
+    asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(tc::smem_u32(bar)), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void copy_box(uint32_t dst, const CUtensorMap* map, int x, int y, int z, int w, uint64_t* bar) {
+    asm volatile("cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];"
+                 ::"r"(dst), "l"(map), "r"(x), "r"(y), "r"(z), "r"(w), "r"(tc::smem_u32(bar))
+                 : "memory");
+}
+__device__ __forceinline__ void fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+
+// V is [position][column]: the product's N runs along a row.  64 columns per 128-byte row; the next 64 a panel further on, the next
+// eight positions 1024 bytes.
+__device__ __forceinline__ uint64_t desc_across(uint32_t at, int panel) {
+    return (uint64_t)((at & 0x3FFFFu) >> 4) | ((uint64_t)(panel >> 4) << 16) | ((uint64_t)(1024 >> 4) << 32) | (1ull << 46) | (2ull << 61);
+}
+__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t add) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(add) : "memory");
+}
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t add) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"(add) : "memory");
+}
+#define HQM_R8(r, i) "=r"(r[i]), "=r"(r[i + 1]), "=r"(r[i + 2]), "=r"(r[i + 3]), "=r"(r[i + 4]), "=r"(r[i + 5]), "=r"(r[i + 6]), "=r"(r[i + 7])
+#define HQM_S8(r, i) "r"(r[i]), "r"(r[i + 1]), "r"(r[i + 2]), "r"(r[i + 3]), "r"(r[i + 4]), "r"(r[i + 5]), "r"(r[i + 6]), "r"(r[i + 7])
+__device__ __forceinline__ void tmem_load32(uint32_t* r, uint32_t at) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,"
+        "%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+        : HQM_R8(r, 0), HQM_R8(r, 8), HQM_R8(r, 16), HQM_R8(r, 24) : "r"(at));
+}
+__device__ __forceinline__ void tmem_load16(uint32_t* r, uint32_t at) {
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+                 : HQM_R8(r, 0), HQM_R8(r, 8) : "r"(at));
+}
+__device__ __forceinline__ void tmem_store16(uint32_t at, const uint32_t* r) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%16], {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15};" ::HQM_S8(r, 0),
+                 HQM_S8(r, 8), "r"(at) : "memory");
+}
+__device__ __forceinline__ void loads_done() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void stores_done() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+template <int D, bool F16>
+__global__ void __launch_bounds__(THREADS, 1) attn_tiles_kernel(const __grid_constant__ CUtensorMap qm, const __grid_constant__ CUtensorMap km,
+                                                                const __grid_constant__ CUtensorMap vm, const __grid_constant__ Args a,
+                                                                int* error_flag) {
+    extern __shared__ __align__(1024) unsigned char raw[];
+    using S = Shared<D>;
+    S& sh = *reinterpret_cast<S*>(raw);
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int per_tile = 128 / a.group, per = 2 * per_tile;        // tokens
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < RING; ++i) {
+            tc::mbar_init(&sh.full[i], 1);
+            tc::mbar_init(&sh.empty[i], 1);
+        }
+        tc::mbar_init(&sh.q_full, 1);
+        tc::mbar_init(&sh.q_empty, 1);
+        for (int t = 0; t < 2; ++t) {
+            tc::mbar_init(&sh.s_full[t], 1);
+            tc::mbar_init(&sh.p_full[t], 4);
+            tc::mbar_init(&sh.o_done[t], 1);
+        }
+        for (int i = 0; i < PARTS; ++i) {
+            tc::mbar_init(&sh.part_full[i], 1);
+            tc::mbar_init(&sh.part_empty[i], 10);
+        }
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (warp == 8) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(tc::smem_u32(&sh.tmem)), "r"(512u) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    grid_launch_dependents();
+    grid_dependency_wait();
+    fence_before();
+    __syncthreads();
+    fence_after();
+    const uint32_t tmem = sh.tmem;
+    Patience patience;
+    uint32_t parts = 0;                                            // parts taken
+    // The next part; false: there is none.  A warp takes it as a whole, and is done with `sh.parts` when it returns.
+    Part w;
+    auto next = [&]() {
+        const int i = parts % PARTS;
+        patience.wait(&sh.part_full[i], (parts / PARTS) & 1);
+        ++parts;
+        w = sh.parts[i];
+        __syncwarp();
+        if (lane == 0) tc::mbar_arrive(&sh.part_empty[i]);
+        return patience.ok && w.tokens > 0;
+    };
+    constexpr uint32_t O_AT = 256;                                 // columns: S 0, 128; O 256, 384
+    if (warp < 8) {
+        // ---- weights: thread = row ----
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(REGS_WEIGHTS));
+        const int t = warp >> 2, r = threadIdx.x & 127;
+        const uint32_t mine = tmem + ((uint32_t)(warp & 3) << 21);
+        const uint32_t s_at = mine + 128 * t, o_at = mine + O_AT + 128 * t;
+        const int tok = t * per_tile + r / a.group;                // within the unit
+        uint32_t blocks_done = 0;
+        while (next()) {
+            if (w.tokens <= t * per_tile) continue;
+            const bool valid = r < per_tile * a.group && tok < w.tokens;
+            const int limit = valid ? min(w.sees + tok, w.kv) : w.kv;          // positions that the row sees
+            float m = -INFINITY, l = 0.f;
+            for (int j = w.j0; j < w.j1; ++j, ++blocks_done) {
+                patience.wait(&sh.s_full[t], blocks_done & 1);
+                fence_after();
+                uint32_t s[KEYS];
+#pragma unroll
+                for (int c = 0; c < 4; ++c) tmem_load32(s + 32 * c, s_at + 32 * c);
+                loads_done();
+                const int seen = limit - j * KEYS;
+                if (__any_sync(0xffffffffu, seen < KEYS)) {
+#pragma unroll
+                    for (int i = 0; i < KEYS; ++i) s[i] = i < seen ? s[i] : 0xff800000u;
+                }
+                float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+                for (int i = 0; i < KEYS; i += 8)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) top[e] = fmaxf(top[e], fmaxf(__uint_as_float(s[i + 2 * e]), __uint_as_float(s[i + 2 * e + 1])));
+                const float block_top = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * a.scale_log2;
+                const bool raise = block_top > m + SLACK || (m == -INFINITY && block_top > m);
+                if (__any_sync(0xffffffffu, raise)) {
+                    const float to = fmaxf(m, block_top);
+                    const float f = to == m ? 1.f : ex2(m - to);
+                    m = to;
+                    l *= f;
+                    if (j > w.j0) {
+                        patience.wait(&sh.o_done[t], (blocks_done - 1) & 1);
+                        fence_after();
+#pragma unroll 1
+                        for (int c = 0; c < D; c += 16) {
+                            uint32_t o[16];
+                            tmem_load16(o, o_at + c);
+                            loads_done();
+#pragma unroll
+                            for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * f);
+                            tmem_store16(o_at + c, o);
+                        }
+                    }
+                }
+                const float base = m == -INFINITY ? 0.f : -m;
+                float sum[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int c = 0; c < KEYS; c += 32) {
+                    uint32_t p[16];
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) {
+                        const float x = ex2(fmaf(__uint_as_float(s[c + 2 * i]), a.scale_log2, base));
+                        const float y = ex2(fmaf(__uint_as_float(s[c + 2 * i + 1]), a.scale_log2, base));
+                        sum[i & 1] += x;
+                        sum[2 + (i & 1)] += y;
+                        p[i] = pack2(x, y, F16);
+                    }
+                    tmem_store16(s_at + c / 2, p);
+                }
+                l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+                stores_done();
+                fence_before();
+                __syncwarp();
+                if (lane == 0) tc::mbar_arrive(&sh.p_full[t]);
+            }
+            // ---- the part's result ----
+            patience.wait(&sh.o_done[t], (blocks_done - 1) & 1);
+            fence_after();
+            const bool whole = w.whole == 1;
+            const float inv = m == -INFINITY ? 0.f : 1.f / l;
+            const int64_t row = ((int64_t)(w.q_row + tok) * a.n_kv + w.head) * a.group + r % a.group;
+            const int pr = t * per_tile * a.group + r;
+            float* piece = piece_at<D>(a, blockIdx.x, w.whole >> 1);
+            if (valid && !whole) {
+                piece[a.piece_rows * D + pr] = m;
+                piece[a.piece_rows * (D + 1) + pr] = l;
+            }
+#pragma unroll 1
+            for (int c = 0; c < D; c += 32) {
+                uint32_t o[32];
+                tmem_load32(o, o_at + c);
+                loads_done();
+                if (!valid) continue;
+                if (whole) {
+                    uint4* dst = reinterpret_cast<uint4*>(a.out + row * D + c);
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        uint32_t v[4];
+#pragma unroll
+                        for (int e = 0; e < 4; ++e)
+                            v[e] = pack2(__uint_as_float(o[8 * i + 2 * e]) * inv, __uint_as_float(o[8 * i + 2 * e + 1]) * inv, F16);
+                        dst[i] = make_uint4(v[0], v[1], v[2], v[3]);
+                    }
+                } else {
+                    uint4* dst = reinterpret_cast<uint4*>(piece + pr * D + c);
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) dst[i] = make_uint4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
+                }
+            }
+            fence_before();
+        }
+    } else {
+        // (A role's code must not come together with one of another number: the compiler counts on the smaller.)
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(REGS_OTHERS));
+        if (warp == 9) {
+            // ---- copies ----
+            const int rows = a.table ? min(1 << a.page_shift, KEYS) : KEYS;
+            const int boxes = KEYS / rows;
+            const uint32_t q_bytes = (uint32_t)(S::HALVES * per_tile * a.group * 128);
+            uint32_t at = 0, units = 0;
+            while (next()) {
+                const int32_t* table = a.table + (int64_t)w.table_row * a.table_stride;
+                for (int j = w.j0; j < w.j1; ++j) {
+                    const int key = j * KEYS + lane * rows;            // of box `lane`; there are eight at the most
+                    const int live = min(boxes, (max(w.kv - j * KEYS, 0) + rows - 1) / rows);
+                    int row = w.kv_row + key, page = 0;
+                    if (a.table && lane < live) {
+                        page = min((uint32_t)table[key >> a.page_shift], (uint32_t)a.n_pages);      // outside the pool: zeros
+                        row = key & ((1 << a.page_shift) - 1);
+                    }
+                    for (int kv = 0; kv < 2; ++kv, ++at) {
+                        const int slot = at % RING;
+                        if (at >= RING) patience.wait(&sh.empty[slot], (at / RING - 1) & 1);
+                        patience.ok = __all_sync(0xffffffffu, patience.ok);
+                        if (patience.ok) {
+                            if (lane == 0) expect(&sh.full[slot], (uint32_t)live * rows * 128 * S::HALVES);
+                            __syncwarp();
+                            if (lane < live)
+#pragma unroll
+                                for (int h = 0; h < S::HALVES; ++h)
+                                    copy_box(tc::smem_u32(sh.ring[slot] + h * S::PANEL + lane * rows * 128), kv ? &vm : &km, 64 * h, row, w.head, page,
+                                             &sh.full[slot]);
+                        }
+                        __syncwarp();
+                    }
+                    if (j == w.j0) {
+                        // Q behind the first block: what the unit before still multiplies with it does not hold that one up
+                        if (units > 0) patience.wait(&sh.q_empty, (units - 1) & 1);
+                        patience.ok = __all_sync(0xffffffffu, patience.ok);
+                        const int tiles = w.tokens > per_tile ? 2 : 1;
+                        if (patience.ok) {
+                            if (lane == 0) {
+                                expect(&sh.q_full, tiles * q_bytes);
+                                for (int t = 0; t < tiles; ++t)
+#pragma unroll
+                                    for (int h = 0; h < S::HALVES; ++h)
+                                        copy_box(tc::smem_u32(sh.q[t] + h * S::PANEL), &qm, 64 * h, 0, w.head, w.q_row + t * per_tile, &sh.q_full);
+                            }
+                            ++units;
+                        }
+                        __syncwarp();
+                    }
+                }
+            }
+            // no copy may be on its way when the CTA ends
+            Patience last;
+            for (uint32_t k = at < RING ? 0 : at - RING; k < at; ++k) last.wait(&sh.full[k % RING], (k / RING) & 1);
+            if (units > 0) last.wait(&sh.q_full, (units - 1) & 1);
+        } else if (warp == 8) {
+            // ---- products ----
+            const uint32_t type = F16 ? 0u : (1u << 7) | (1u << 10);
+            const uint32_t idesc_s = (1u << 4) | type | ((KEYS / 8) << 17) | ((128u >> 4) << 24);
+            const uint32_t idesc_o = (1u << 4) | type | (1u << 16) | ((D / 8) << 17) | ((128u >> 4) << 24);
+            uint32_t at = 0, units = 0, p_seen[2] = {0, 0};
+            auto scores = [&](int t, int slot) {                       // S_t = Q_t K^T
+                if (lane == 0) {
+                    const uint64_t qa = tc::smem_desc_sw128(tc::smem_u32(sh.q[t])), kb = tc::smem_desc_sw128(tc::smem_u32(sh.ring[slot]));
+#pragma unroll
+                    for (int k = 0; k < D / 16; ++k) {
+                        const uint64_t off = ((k >> 2) * S::PANEL + (k & 3) * 32) >> 4;
+                        mma_ss(tmem + 128 * t, qa + off, kb + off, idesc_s, k > 0);
+                    }
+                    tc::umma_commit(&sh.s_full[t]);
+                }
+                __syncwarp();
+            };
+            while (next()) {
+                const int tiles = w.tokens > per_tile ? 2 : 1;
+                patience.wait(&sh.full[at % RING], (at / RING) & 1);
+                patience.wait(&sh.q_full, units & 1);
+                ++units;
+                fence_after();
+                for (int t = 0; t < tiles; ++t) scores(t, at % RING);
+                if (lane == 0) {
+                    tc::umma_commit(&sh.empty[at % RING]);
+                    if (w.j1 - w.j0 == 1) tc::umma_commit(&sh.q_empty);
+                }
+                for (int j = w.j0; j < w.j1; ++j, at += 2) {
+                    const int vs = (at + 1) % RING, ks = (at + 2) % RING;
+                    const bool more = j + 1 < w.j1;
+                    patience.wait(&sh.full[vs], ((at + 1) / RING) & 1);
+                    const int live = w.kv - j * KEYS;                  // positions of the block that belong to the sequence
+                    if (live < KEYS) {
+                        // behind them lies anything, also NaN, which no weight of zero takes away
+                        for (int i = max(live, 0) * 8 + lane; i < KEYS * 8; i += 32)
+#pragma unroll
+                            for (int h = 0; h < S::HALVES; ++h) *reinterpret_cast<uint4*>(sh.ring[vs] + h * S::PANEL + i * 16) = make_uint4(0, 0, 0, 0);
+                        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                        __syncwarp();
+                    }
+                    for (int t = 0; t < tiles; ++t) {
+                        patience.wait(&sh.p_full[t], p_seen[t]++ & 1);
+                        fence_after();
+                        if (lane == 0) {
+                            const uint64_t vb = desc_across(tc::smem_u32(sh.ring[vs]), S::PANEL);
+#pragma unroll
+                            for (int k = 0; k < KEYS / 16; ++k)
+                                mma_ts(tmem + O_AT + 128 * t, tmem + 128 * t + 8 * k, vb + ((k * 16 * 128) >> 4), idesc_o, j > w.j0 || k > 0);
+                            tc::umma_commit(&sh.o_done[t]);
+                        }
+                        __syncwarp();
+                        if (more) {
+                            if (t == 0) {
+                                patience.wait(&sh.full[ks], ((at + 2) / RING) & 1);
+                                fence_after();
+                            }
+                            scores(t, ks);
+                        }
+                    }
+                    if (lane == 0) {
+                        tc::umma_commit(&sh.empty[vs]);
+                        if (more) {
+                            tc::umma_commit(&sh.empty[ks]);
+                            if (j + 2 == w.j1) tc::umma_commit(&sh.q_empty);
+                        }
+                    }
+                }
+            }
+        } else if (warp == 10) {
+            // ---- the list ----
+            const Run run = find_run(a, per, KEYS);
+            Walk walk(a, run, per, KEYS);
+            bool cut = false, some;
+            uint32_t n = 0;
+            do {
+                some = walk.next();
+                if (n >= PARTS) patience.wait(&sh.part_empty[n % PARTS], (n / PARTS - 1) & 1);
+                if (some && walk.j0 == 0 && walk.j1 < walk.blocks) {
+                    cut = true;
+                    if (lane == 0) write_record(a, &walk, run.share);
+                }
+                if (lane == 0) {
+                    Part p{};
+                    if (some)
+                        p = Part{walk.tokens(), walk.s.q0 + walk.first_token(), walk.h, walk.s.before + walk.first_token() + 1, walk.s.kv, walk.j0,
+                                 walk.j1, walk.s.q0, walk.b, walk.whole() ? 1 : 2 * (walk.j0 == 0)};
+                    sh.parts[n % PARTS] = p;
+                    tc::mbar_arrive(&sh.part_full[n % PARTS]);
+                }
+                __syncwarp();
+                ++n;
+            } while (some);
+            if (!cut && lane == 0) write_record(a, nullptr, run.share);
+        }
+    }
+    if (!patience.ok && lane == 0 && error_flag) atomicExch(error_flag, 1);
+    fence_before();
+    __syncthreads();
+    if (warp == 8) {
+        fence_after();
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u) : "memory");
+    }
+}
+
+template <int D, bool F16>
+int tiles_launch(const Args& a, const CUtensorMap& qm, const CUtensorMap& km, const CUtensorMap& vm, int ctas, cudaStream_t st) {
+    constexpr size_t bytes = sizeof(Shared<D>);
+    static SharedLimits limits;
+    if (!allow_shared(attn_tiles_kernel<D, F16>, limits, bytes)) {
+        set_error("attention: a CTA cannot have %zu bytes of shared memory", bytes);
+        return HQM_ERR_CUDA;
+    }
+    HQM_CUDA(launch_overlapped(attn_tiles_kernel<D, F16>, ctas, THREADS, bytes, st, qm, km, vm, a, tc_error_ptr()));
+    HQM_LAUNCH_CHECK();
+    return HQM_OK;
+}
+
+}  // namespace
+
+int launch_tiles(const Args& a, const CUtensorMap& qm, const CUtensorMap& km, const CUtensorMap& vm, int ctas, int D, bool f16, cudaStream_t st) {
+    if (D == 128) return f16 ? tiles_launch<128, true>(a, qm, km, vm, ctas, st) : tiles_launch<128, false>(a, qm, km, vm, ctas, st);
+    return f16 ? tiles_launch<64, true>(a, qm, km, vm, ctas, st) : tiles_launch<64, false>(a, qm, km, vm, ctas, st);
+}
+
+}  // namespace attn
+}  // namespace hqm

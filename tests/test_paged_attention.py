@@ -92,7 +92,7 @@ class Problem:
         return reference(self.q, self.ks, self.vs, self.cu, self.q.shape[-1] ** -0.5 if scale is None else scale)
 
 
-HEADS = [(32, 8), (4, 4), (16, 2), (12, 2), (14, 2), (16, 1), (9, 3)]
+HEADS = [(32, 8), (4, 4), (16, 2), (12, 2), (14, 2), (16, 1), (9, 3), (40, 1), (128, 1)]
 
 
 @pytest.mark.parametrize("H,n_kv", HEADS)

@@ -240,7 +240,8 @@ def test_the_library_refuses_what_it_cannot_do():
                          (dict(table_stride=3), "pages"), (dict(max_pages=0), "pages"), (dict(pages=1 << 28), "pages"),
                          (dict(max_pages=1 << 28, table_stride=1 << 28), "pages"), (dict(q=0), "null"), (dict(kv_lens=0), "null"),
                          (dict(q_token=513), "16-byte"), (dict(k_page=4100), "16-byte"), (dict(v=4104), "16-byte"), (dict(tokens=-1), "tokens"),
-                         (dict(tokens=1 << 31), "tokens"), (dict(max_new=-1), "at most"), (dict(scale=float("nan")), "scale")):
+                         (dict(tokens=1 << 31), "tokens"), (dict(max_new=-1), "at most"), (dict(scale=float("nan")), "scale"),
+                         (dict(scale=0.0), "positive"), (dict(n_heads=258), "query heads")):
         call = _cabi.HqmAttention(**dict(ok, **change))
         assert lib.hqm_paged_attention(C.byref(call), some, 1 << 40, None) == _cabi.HQM_ERR_ARG, change
         assert word in _cabi.last_error(), (change, _cabi.last_error())
