@@ -65,7 +65,7 @@ int check(const hqm_attention* c, bool paged, const char* what) {
 
 // Whether a unit of attn_few.cu holds all new tokens of any sequence.
 bool few_rows(const hqm_attention* c) { return (int64_t)c->max_new * (c->n_heads / c->n_kv_heads) <= FEW_TILE; }
-int rows_of_piece(const hqm_attention* c) { return few_rows(c) ? FEW_TILE : 2 * TILE_KEYS; }
+int rows_of_piece(const hqm_attention* c) { return few_rows(c) ? FEW_TILE : TILE_ROWS; }
 
 int run(const hqm_attention* c, bool paged, const char* what, void* scratch, size_t scratch_bytes, void* stream) {
     if (int rc = check(c, paged, what)) return rc;

@@ -5,8 +5,9 @@
 // key/value head are rows of the same tile (row = token * group + head), so that keys and values are read once for all of them.
 //
 // The work is a list of units (sequence, key/value head, tile of rows), each of as many blocks of keys as its last row sees, at
-// least one.  The list's blocks are cut into equal runs, one per CTA, wherever that falls: every CTA finds its run from the
-// lengths in device memory, so the host needs no length and a captured graph follows them.  A unit that a cut goes through leaves
+// least one.  The list is cut into runs of equal cost, one per CTA, wherever that falls; a unit costs its blocks and, in front of
+// them, `extra` blocks for its beginning and end (a cut in there falls in front of the unit).  Every CTA finds its run from
+// the lengths in device memory, so the host needs no length and a captured graph follows them.  A unit that a cut goes through leaves
 // unnormalised sums with their maximum and total (a "piece") per CTA, which attn_join adds in the order of the CTAs: the same
 // bits for the same lengths, whichever CTA ends first.
 #pragma once
@@ -58,24 +59,29 @@ struct Seq {
     int kv;                        // positions that can be read
     int before;                    // kv - n: what token 0 sees, less one
     int tiles, per;                // tiles of rows, tokens per tile
-    int block;                     // keys per block
+    int block, extra;              // keys per block, blocks that a unit costs beside its own
     __host__ __device__ int blocks(int tile) const {
         const int seen = before + min((tile + 1) * per, n);
         return max(1, (seen + block - 1) / block);
     }
-    // blocks of tiles 0 .. count - 1
+    // cost of tiles 0 .. count - 1
     __host__ __device__ int64_t prefix(int count) const {
         const int whole = min(count, tiles - 1);               // tiles of `per` tokens
         int empty = 0;                                         // of them, the ones that see nothing: one block each
         if (before < 0) empty = min(whole, (-before) / per);
-        int64_t sum = empty + floor_sum(whole - empty, block, per, (int64_t)before + (int64_t)(empty + 1) * per + block - 1);
+        int64_t sum = (int64_t)count * extra + empty + floor_sum(whole - empty, block, per, (int64_t)before + (int64_t)(empty + 1) * per + block - 1);
         if (count >= tiles && tiles > 0) sum += blocks(tiles - 1);
         return sum;
     }
     __host__ __device__ int64_t total() const { return prefix(tiles); }
 };
 
-__device__ __forceinline__ Seq load_seq(const Args& a, int b, int per, int block) {
+// How a kernel cuts the work.
+struct Cut {
+    int per, block, extra;         // tokens per tile, keys per block, blocks beside a unit's own
+};
+
+__device__ __forceinline__ Seq load_seq(const Args& a, int b, const Cut& c) {
     Seq s;
     const int lo = min(max(a.cu[b], 0), a.T), hi = min(max(a.cu[b + 1], lo), a.T);
     s.q0 = lo;
@@ -83,27 +89,28 @@ __device__ __forceinline__ Seq load_seq(const Args& a, int b, int per, int block
     s.kv = s.n;
     if (a.table) s.kv = (int)min((int64_t)max(a.kv_lens[b], 0), (int64_t)a.max_pages << a.page_shift);
     s.before = s.kv - s.n;
-    s.per = per;
-    s.block = block;
-    s.tiles = (s.n + per - 1) / per;
+    s.per = c.per;
+    s.block = c.block;
+    s.extra = c.extra;
+    s.tiles = (s.n + c.per - 1) / c.per;
     return s;
 }
 
 // Where a CTA's run of blocks begins, and how long it is.
 struct Run {
-    int64_t share;                 // blocks of every run (the last one may have fewer)
-    int64_t left;                  // blocks of this one
+    int64_t share;                 // cost of every run (the last one may have less)
+    int64_t left;                  // of this one
     int b, h, tile;
-    int skip;                      // blocks of its first unit that belong to earlier CTAs
+    int skip;                      // cost of its first unit that lies in front of the run
 };
 
 // Called by one whole warp; every lane gets the run.
-__device__ inline Run find_run(const Args& a, int per, int block) {
+__device__ inline Run find_run(const Args& a, const Cut& c) {
     const int lane = threadIdx.x & 31;
     int64_t total = 0;
     for (int b0 = 0; b0 < a.B; b0 += 32) {
         int64_t w = 0;
-        if (b0 + lane < a.B) w = load_seq(a, b0 + lane, per, block).total() * a.n_kv;
+        if (b0 + lane < a.B) w = load_seq(a, b0 + lane, c).total() * a.n_kv;
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) w += __shfl_xor_sync(0xffffffffu, w, o);
         total += w;
@@ -117,7 +124,7 @@ __device__ inline Run find_run(const Args& a, int per, int block) {
     int64_t base = 0;
     for (int b0 = 0; b0 < a.B; b0 += 32) {
         int64_t w = 0;
-        if (b0 + lane < a.B) w = load_seq(a, b0 + lane, per, block).total() * a.n_kv;
+        if (b0 + lane < a.B) w = load_seq(a, b0 + lane, c).total() * a.n_kv;
         int64_t sum = w;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
@@ -129,7 +136,7 @@ __device__ inline Run find_run(const Args& a, int per, int block) {
             const int src = __ffs(past) - 1;
             r.b = b0 + src;
             const int64_t off = lo - (base + __shfl_sync(0xffffffffu, sum - w, src));
-            const Seq s = load_seq(a, r.b, per, block);
+            const Seq s = load_seq(a, r.b, c);
             const int64_t one = s.total();
             r.h = (int)(off / one);
             const int64_t in = off - r.h * one;
@@ -152,30 +159,33 @@ __device__ inline Run find_run(const Args& a, int per, int block) {
 // A CTA's walk through its run: every part of a unit that it works on, in order.  All threads that walk it see the same.
 struct Walk {
     const Args& a;
+    Cut cut;
     Seq s;
     int64_t left;
     int b, h, tile, skip;
     int j0, j1, blocks;            // the part: blocks j0 .. j1 - 1 of `blocks`
-    __device__ Walk(const Args& args, const Run& r, int per, int block) : a(args), left(r.left), b(r.b), h(r.h), tile(r.tile), skip(r.skip) {
-        if (left > 0) s = load_seq(a, b, per, block);
+    __device__ Walk(const Args& args, const Run& r, const Cut& c) : a(args), cut(c), left(r.left), b(r.b), h(r.h), tile(r.tile), skip(r.skip) {
+        if (left > 0) s = load_seq(a, b, cut);
     }
     __device__ bool next() {       // false: done
-        if (left <= 0) return false;
-        if (tile == s.tiles) {
-            tile = 0;
-            if (++h == a.n_kv) {
-                h = 0;
-                do s = load_seq(a, ++b, s.per, s.block);
-                while (s.tiles == 0);
+        while (left > 0) {
+            if (tile == s.tiles) {
+                tile = 0;
+                if (++h == a.n_kv) {
+                    h = 0;
+                    do s = load_seq(a, ++b, cut);
+                    while (s.tiles == 0);
+                }
             }
+            blocks = s.blocks(tile++);
+            const int end = (int)min((int64_t)(blocks + s.extra), skip + left);
+            left -= end - skip;
+            j0 = max(skip - s.extra, 0);
+            j1 = max(end - s.extra, 0);
+            skip = 0;
+            if (j1 > j0) return true;
         }
-        blocks = s.blocks(tile);
-        j0 = skip;
-        j1 = (int)min((int64_t)blocks, j0 + left);
-        left -= j1 - j0;
-        skip = 0;
-        ++tile;
-        return true;
+        return false;
     }
     // the part's tile is tile - 1 from here on
     __device__ int first_token() const { return (tile - 1) * s.per; }
@@ -230,7 +240,8 @@ int launch_tiles(const Args& a, const CUtensorMap& qm, const CUtensorMap& km, co
 
 constexpr int FEW_TILE = 16;       // rows of a unit of attn_few.cu
 constexpr int FEW_KEYS = 64;       // positions of a block there
-constexpr int TILE_KEYS = 128;     // and in attn_tiles.cu
+constexpr int TILE_ROWS = 256;     // rows of a unit of attn_tiles.cu
+constexpr int TILE_KEYS = 128;      // positions of a block there
 constexpr int MAX_GROUP = 128;     // query heads per key/value head: the rows of a tile
 
 }  // namespace attn

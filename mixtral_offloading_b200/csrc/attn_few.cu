@@ -19,6 +19,7 @@ namespace {
 constexpr int CONSUMERS = 8;
 constexpr int THREADS = 32 * (CONSUMERS + 1);
 constexpr int STAGES = 4;
+constexpr int UNIT_EXTRA = 1;          // what a unit costs beside its blocks, in blocks
 
 template <int D>
 struct Shared {
@@ -64,7 +65,7 @@ __global__ void __launch_bounds__(THREADS, 1) attn_few_kernel(const __grid_const
     using S = Shared<D>;
     S& sh = *reinterpret_cast<S*>(raw);
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const int per = FEW_TILE / a.group;
+    const Cut how{FEW_TILE / a.group, FEW_KEYS, UNIT_EXTRA};
     if (threadIdx.x == 0) {
         for (int i = 0; i < STAGES; ++i) {
             tc::mbar_init(&sh.full[i], 1);
@@ -75,12 +76,12 @@ __global__ void __launch_bounds__(THREADS, 1) attn_few_kernel(const __grid_const
     grid_launch_dependents();
     grid_dependency_wait();
     if (warp == 0) {
-        const Run r = find_run(a, per, FEW_KEYS);
+        const Run r = find_run(a, how);
         if (lane == 0) sh.run = r;
     }
     __syncthreads();
     const Run run = sh.run;
-    Walk w(a, run, per, FEW_KEYS);
+    Walk w(a, run, how);
     bool ok = true;
     if (warp == CONSUMERS) {
         // ---- the copies: lane i brings box i of a stage ----

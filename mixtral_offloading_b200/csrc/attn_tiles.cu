@@ -10,12 +10,14 @@
 // cores work on the other tile's products.
 //
 // Warps 0-3: weights of tile 0, 4-7: of tile 1, 8: issues the products, 9: copies (cp.async.bulk.tensor; Q once per unit, K and
-// V of every block through a ring of five buffers, of a paged cache a copy per page); 10: walks the list of units; 11
+// V of every block through a ring of five buffers, of a paged cache a copy per page), 10: walks the list of units; 11
 // only completes the warpgroup.
 //
 // The maximum m that a row's weights refer to is raised only when a block exceeds it by more than 2^8: O, which lies in tensor
 // memory, is rescaled a few times per unit instead of once per block, weights grow to 256 at the most, and l and O mean the same
 // whatever m is.
+#include <type_traits>
+
 #include "attn.cuh"
 #include "shared_limit.h"
 #include "tc_common.cuh"
@@ -27,10 +29,12 @@ namespace {
 constexpr int KEYS = TILE_KEYS;
 constexpr int RING = 5;
 // Three warpgroups of 168 registers a thread at the launch (64512): the two that form weights take 216, the third keeps 72.
-constexpr int THREADS = 384;
+constexpr int WEIGHT_WARPS = 8, THREADS = 32 * WEIGHT_WARPS + 128;
 constexpr int REGS_WEIGHTS = 216, REGS_OTHERS = 72;
-static_assert(256 * REGS_WEIGHTS + 128 * REGS_OTHERS <= THREADS * 168, "registers of the launch");
+static_assert(32 * WEIGHT_WARPS * REGS_WEIGHTS + 128 * REGS_OTHERS <= THREADS * 168, "registers of the launch");
 constexpr float SLACK = 8.f;
+constexpr int UNIT_EXTRA = 2;         // what a unit costs beside its blocks, in blocks
+constexpr int BY_POLYNOMIAL = 4;      // of 16 pairs of weights
 
 // A part of a unit (Walk), as the warp that walks the list hands it to the others.
 struct Part {
@@ -89,6 +93,54 @@ __device__ __forceinline__ void copy_box(uint32_t dst, const CUtensorMap* map, i
 __device__ __forceinline__ void fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
 
+// Two floats for the packed instructions.
+typedef unsigned long long Pair;
+__device__ __forceinline__ Pair pair(float lo, float hi) {
+    Pair r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
+    return r;
+}
+__device__ __forceinline__ float low(Pair v) { return __uint_as_float((uint32_t)v); }
+__device__ __forceinline__ float high(Pair v) { return __uint_as_float((uint32_t)(v >> 32)); }
+__device__ __forceinline__ Pair fma2(Pair a, Pair b, Pair c) {
+    Pair r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
+}
+__device__ __forceinline__ Pair add2(Pair a, Pair b) {
+    Pair r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    float r;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+    return r;
+}
+
+// 2^x without the special-function unit, x up to 2^7: x = n + f with f in [-1/2, 1/2] (the sum with 1.5 2^23 rounds to n), 2^f by
+// the polynomial of least relative error there, n into the exponent.  Off by 7.5e-5 of the value with degree 3 (bf16 rounds
+// by up to 3.9e-3), by 2.6e-6 with degree 4 (fp16: 4.9e-4).  Below 2^-125 the result is 2^-125.
+template <bool F16>
+__device__ __forceinline__ Pair power2(Pair x) {
+    const Pair magic = pair(12582912.f, 12582912.f), unmagic = pair(-12582912.f, -12582912.f), minus = pair(-1.f, -1.f);
+    x = pair(fmaxf(low(x), -125.f), fmaxf(high(x), -125.f));
+    const Pair t = add2(x, magic), n = add2(t, unmagic), f = fma2(n, minus, x);
+    Pair p;
+    if constexpr (F16) {
+        p = fma2(pair(0.00957007613f, 0.00957007613f), f, pair(0.0559178926f, 0.0559178926f));
+        p = fma2(p, f, pair(0.240247458f, 0.240247458f));
+        p = fma2(p, f, pair(0.693121791f, 0.693121791f));
+        p = fma2(p, f, pair(0.999999285f, 0.999999285f));
+    } else {
+        p = fma2(pair(0.0551717728f, 0.0551717728f), f, pair(0.242611378f, 0.242611378f));
+        p = fma2(p, f, pair(0.693260968f, 0.693260968f));
+        p = fma2(p, f, pair(0.999927998f, 0.999927998f));
+    }
+    return pair(__uint_as_float(__float_as_uint(low(p)) + (__float_as_uint(low(t)) << 23)),
+                __uint_as_float(__float_as_uint(high(p)) + (__float_as_uint(high(t)) << 23)));
+}
+
 // V is [position][column]: the product's N runs along a row.  64 columns per 128-byte row; the next 64 a panel further on, the next
 // eight positions 1024 bytes.
 __device__ __forceinline__ uint64_t desc_across(uint32_t at, int panel) {
@@ -120,8 +172,24 @@ __device__ __forceinline__ void tmem_store16(uint32_t at, const uint32_t* r) {
     asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%16], {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15};" ::HQM_S8(r, 0),
                  HQM_S8(r, 8), "r"(at) : "memory");
 }
-__device__ __forceinline__ void loads_done() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void tmem_store8(uint32_t at, const uint32_t* r) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%8], {%0,%1,%2,%3,%4,%5,%6,%7};" ::HQM_S8(r, 0), "r"(at) : "memory");
+}
+// The loads of r have arrived.  (The registers go through, so that no use of them moves in front.)
+#define HQM_B8(r, i) "+r"(r[i]), "+r"(r[i + 1]), "+r"(r[i + 2]), "+r"(r[i + 3]), "+r"(r[i + 4]), "+r"(r[i + 5]), "+r"(r[i + 6]), "+r"(r[i + 7])
+__device__ __forceinline__ void loads_done(uint32_t* r) {
+    asm volatile("tcgen05.wait::ld.sync.aligned;" : HQM_B8(r, 0), HQM_B8(r, 8), HQM_B8(r, 16), HQM_B8(r, 24)::"memory");
+}
+__device__ __forceinline__ void loads_done16(uint32_t* r) { asm volatile("tcgen05.wait::ld.sync.aligned;" : HQM_B8(r, 0), HQM_B8(r, 8)::"memory"); }
 __device__ __forceinline__ void stores_done() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+// True in one lane, the same each time.  (The compiler knows this for one lane: behind `lane == 0` it moved the operands of every
+// product into uniform registers one by one, 95 to 125 cycles per instruction instead of 32 or 64.)
+__device__ __forceinline__ bool elected() {
+    uint32_t one;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(one));
+    return one != 0;
+}
 
 template <int D, bool F16>
 __global__ void __launch_bounds__(THREADS, 1) attn_tiles_kernel(const __grid_constant__ CUtensorMap qm, const __grid_constant__ CUtensorMap km,
@@ -131,7 +199,7 @@ __global__ void __launch_bounds__(THREADS, 1) attn_tiles_kernel(const __grid_con
     using S = Shared<D>;
     S& sh = *reinterpret_cast<S*>(raw);
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const int per_tile = 128 / a.group, per = 2 * per_tile;        // tokens
+    const int per_tile = 128 / a.group;                            // tokens
     if (threadIdx.x == 0) {
         for (int i = 0; i < RING; ++i) {
             tc::mbar_init(&sh.full[i], 1);
@@ -141,16 +209,16 @@ __global__ void __launch_bounds__(THREADS, 1) attn_tiles_kernel(const __grid_con
         tc::mbar_init(&sh.q_empty, 1);
         for (int t = 0; t < 2; ++t) {
             tc::mbar_init(&sh.s_full[t], 1);
-            tc::mbar_init(&sh.p_full[t], 4);
+            tc::mbar_init(&sh.p_full[t], WEIGHT_WARPS / 2);
             tc::mbar_init(&sh.o_done[t], 1);
         }
         for (int i = 0; i < PARTS; ++i) {
             tc::mbar_init(&sh.part_full[i], 1);
-            tc::mbar_init(&sh.part_empty[i], 10);
+            tc::mbar_init(&sh.part_empty[i], WEIGHT_WARPS + 2);
         }
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
-    if (warp == 8) {
+    if (warp == WEIGHT_WARPS) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(tc::smem_u32(&sh.tmem)), "r"(512u) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     }
@@ -174,7 +242,7 @@ __global__ void __launch_bounds__(THREADS, 1) attn_tiles_kernel(const __grid_con
         return patience.ok && w.tokens > 0;
     };
     constexpr uint32_t O_AT = 256;                                 // columns: S 0, 128; O 256, 384
-    if (warp < 8) {
+    if (warp < WEIGHT_WARPS) {
         // ---- weights: thread = row ----
         asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(REGS_WEIGHTS));
         const int t = warp >> 2, r = threadIdx.x & 127;
@@ -192,8 +260,9 @@ __global__ void __launch_bounds__(THREADS, 1) attn_tiles_kernel(const __grid_con
                 fence_after();
                 uint32_t s[KEYS];
 #pragma unroll
-                for (int c = 0; c < 4; ++c) tmem_load32(s + 32 * c, s_at + 32 * c);
-                loads_done();
+                for (int c = 0; c < KEYS; c += 32) tmem_load32(s + c, s_at + c);
+#pragma unroll
+                for (int c = 0; c < KEYS; c += 32) loads_done(s + c);
                 const int seen = limit - j * KEYS;
                 if (__any_sync(0xffffffffu, seen < KEYS)) {
 #pragma unroll
@@ -203,8 +272,8 @@ __global__ void __launch_bounds__(THREADS, 1) attn_tiles_kernel(const __grid_con
 #pragma unroll
                 for (int i = 0; i < KEYS; i += 8)
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) top[e] = fmaxf(top[e], fmaxf(__uint_as_float(s[i + 2 * e]), __uint_as_float(s[i + 2 * e + 1])));
-                const float block_top = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * a.scale_log2;
+                    for (int e = 0; e < 4; ++e) top[e] = max3(top[e], __uint_as_float(s[i + 2 * e]), __uint_as_float(s[i + 2 * e + 1]));
+                const float block_top = fmaxf(max3(top[0], top[1], top[2]), top[3]) * a.scale_log2;
                 const bool raise = block_top > m + SLACK || (m == -INFINITY && block_top > m);
                 if (__any_sync(0xffffffffu, raise)) {
                     const float to = fmaxf(m, block_top);
@@ -218,7 +287,7 @@ __global__ void __launch_bounds__(THREADS, 1) attn_tiles_kernel(const __grid_con
                         for (int c = 0; c < D; c += 16) {
                             uint32_t o[16];
                             tmem_load16(o, o_at + c);
-                            loads_done();
+                            loads_done16(o);
 #pragma unroll
                             for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * f);
                             tmem_store16(o_at + c, o);
@@ -226,25 +295,26 @@ __global__ void __launch_bounds__(THREADS, 1) attn_tiles_kernel(const __grid_con
                     }
                 }
                 const float base = m == -INFINITY ? 0.f : -m;
-                float sum[4] = {0.f, 0.f, 0.f, 0.f};
+                const Pair scale2 = pair(a.scale_log2, a.scale_log2), base2 = pair(base, base);
+                Pair sum[2] = {pair(0.f, 0.f), pair(0.f, 0.f)};
 #pragma unroll
                 for (int c = 0; c < KEYS; c += 32) {
                     uint32_t p[16];
 #pragma unroll
                     for (int i = 0; i < 16; ++i) {
-                        const float x = ex2(fmaf(__uint_as_float(s[c + 2 * i]), a.scale_log2, base));
-                        const float y = ex2(fmaf(__uint_as_float(s[c + 2 * i + 1]), a.scale_log2, base));
-                        sum[i & 1] += x;
-                        sum[2 + (i & 1)] += y;
-                        p[i] = pack2(x, y, F16);
+                        const Pair x = fma2(pair(__uint_as_float(s[c + 2 * i]), __uint_as_float(s[c + 2 * i + 1])), scale2, base2);
+                        const Pair y = (i * BY_POLYNOMIAL) % 16 + BY_POLYNOMIAL >= 16 ? power2<F16>(x) : pair(ex2(low(x)), ex2(high(x)));
+                        sum[i & 1] = add2(sum[i & 1], y);
+                        p[i] = pack2(low(y), high(y), F16);
                     }
                     tmem_store16(s_at + c / 2, p);
                 }
-                l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
                 stores_done();
                 fence_before();
                 __syncwarp();
                 if (lane == 0) tc::mbar_arrive(&sh.p_full[t]);
+                sum[0] = add2(sum[0], sum[1]);
+                l += low(sum[0]) + high(sum[0]);
             }
             // ---- the part's result ----
             patience.wait(&sh.o_done[t], (blocks_done - 1) & 1);
@@ -262,7 +332,7 @@ __global__ void __launch_bounds__(THREADS, 1) attn_tiles_kernel(const __grid_con
             for (int c = 0; c < D; c += 32) {
                 uint32_t o[32];
                 tmem_load32(o, o_at + c);
-                loads_done();
+                loads_done(o);
                 if (!valid) continue;
                 if (whole) {
                     uint4* dst = reinterpret_cast<uint4*>(a.out + row * D + c);
@@ -285,7 +355,7 @@ __global__ void __launch_bounds__(THREADS, 1) attn_tiles_kernel(const __grid_con
     } else {
         // (A role's code must not come together with one of another number: the compiler counts on the smaller.)
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(REGS_OTHERS));
-        if (warp == 9) {
+        if (warp == WEIGHT_WARPS + 1) {
             // ---- copies ----
             const int rows = a.table ? min(1 << a.page_shift, KEYS) : KEYS;
             const int boxes = KEYS / rows;
@@ -339,14 +409,14 @@ __global__ void __launch_bounds__(THREADS, 1) attn_tiles_kernel(const __grid_con
             Patience last;
             for (uint32_t k = at < RING ? 0 : at - RING; k < at; ++k) last.wait(&sh.full[k % RING], (k / RING) & 1);
             if (units > 0) last.wait(&sh.q_full, (units - 1) & 1);
-        } else if (warp == 8) {
+        } else if (warp == WEIGHT_WARPS) {
             // ---- products ----
             const uint32_t type = F16 ? 0u : (1u << 7) | (1u << 10);
             const uint32_t idesc_s = (1u << 4) | type | ((KEYS / 8) << 17) | ((128u >> 4) << 24);
             const uint32_t idesc_o = (1u << 4) | type | (1u << 16) | ((D / 8) << 17) | ((128u >> 4) << 24);
             uint32_t at = 0, units = 0, p_seen[2] = {0, 0};
             auto scores = [&](int t, int slot) {                       // S_t = Q_t K^T
-                if (lane == 0) {
+                if (elected()) {
                     const uint64_t qa = tc::smem_desc_sw128(tc::smem_u32(sh.q[t])), kb = tc::smem_desc_sw128(tc::smem_u32(sh.ring[slot]));
 #pragma unroll
                     for (int k = 0; k < D / 16; ++k) {
@@ -364,7 +434,7 @@ __global__ void __launch_bounds__(THREADS, 1) attn_tiles_kernel(const __grid_con
                 ++units;
                 fence_after();
                 for (int t = 0; t < tiles; ++t) scores(t, at % RING);
-                if (lane == 0) {
+                if (elected()) {
                     tc::umma_commit(&sh.empty[at % RING]);
                     if (w.j1 - w.j0 == 1) tc::umma_commit(&sh.q_empty);
                 }
@@ -372,19 +442,21 @@ __global__ void __launch_bounds__(THREADS, 1) attn_tiles_kernel(const __grid_con
                     const int vs = (at + 1) % RING, ks = (at + 2) % RING;
                     const bool more = j + 1 < w.j1;
                     patience.wait(&sh.full[vs], ((at + 1) / RING) & 1);
+                    if (more) patience.wait(&sh.full[ks], ((at + 2) / RING) & 1);
                     const int live = w.kv - j * KEYS;                  // positions of the block that belong to the sequence
                     if (live < KEYS) {
                         // behind them lies anything, also NaN, which no weight of zero takes away
                         for (int i = max(live, 0) * 8 + lane; i < KEYS * 8; i += 32)
 #pragma unroll
-                            for (int h = 0; h < S::HALVES; ++h) *reinterpret_cast<uint4*>(sh.ring[vs] + h * S::PANEL + i * 16) = make_uint4(0, 0, 0, 0);
+                            for (int h = 0; h < S::HALVES; ++h)
+                                *reinterpret_cast<uint4*>(sh.ring[vs] + h * S::PANEL + i * 16) = make_uint4(0, 0, 0, 0);
                         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                         __syncwarp();
                     }
                     for (int t = 0; t < tiles; ++t) {
                         patience.wait(&sh.p_full[t], p_seen[t]++ & 1);
                         fence_after();
-                        if (lane == 0) {
+                        if (elected()) {
                             const uint64_t vb = desc_across(tc::smem_u32(sh.ring[vs]), S::PANEL);
 #pragma unroll
                             for (int k = 0; k < KEYS / 16; ++k)
@@ -392,27 +464,23 @@ __global__ void __launch_bounds__(THREADS, 1) attn_tiles_kernel(const __grid_con
                             tc::umma_commit(&sh.o_done[t]);
                         }
                         __syncwarp();
-                        if (more) {
-                            if (t == 0) {
-                                patience.wait(&sh.full[ks], ((at + 2) / RING) & 1);
-                                fence_after();
-                            }
-                            scores(t, ks);
-                        }
+                        if (more) scores(t, ks);
                     }
-                    if (lane == 0) {
+                    if (elected()) {
                         tc::umma_commit(&sh.empty[vs]);
                         if (more) {
                             tc::umma_commit(&sh.empty[ks]);
                             if (j + 2 == w.j1) tc::umma_commit(&sh.q_empty);
                         }
                     }
+                    __syncwarp();
                 }
             }
-        } else if (warp == 10) {
+        } else if (warp == WEIGHT_WARPS + 2) {
             // ---- the list ----
-            const Run run = find_run(a, per, KEYS);
-            Walk walk(a, run, per, KEYS);
+            const Cut how{2 * per_tile, KEYS, UNIT_EXTRA};
+            const Run run = find_run(a, how);
+            Walk walk(a, run, how);
             bool cut = false, some;
             uint32_t n = 0;
             do {
@@ -439,7 +507,7 @@ __global__ void __launch_bounds__(THREADS, 1) attn_tiles_kernel(const __grid_con
     if (!patience.ok && lane == 0 && error_flag) atomicExch(error_flag, 1);
     fence_before();
     __syncthreads();
-    if (warp == 8) {
+    if (warp == WEIGHT_WARPS) {
         fence_after();
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u) : "memory");
     }

@@ -10,9 +10,12 @@
 #define PY_SSIZE_T_CLEAN
 #include <Python.h>
 
+#include <algorithm>
+#include <cmath>
 #include <cstring>
 
 #include <ATen/Functions.h>
+#include <ATen/core/LegacyTypeDispatch.h>
 #include <ATen/core/Tensor.h>
 #include <c10/core/InferenceMode.h>
 #include <c10/cuda/CUDAFunctions.h>
@@ -334,6 +337,255 @@ PyObject* expert_addresses(PyObject*, PyObject* const* args, Py_ssize_t n) {
     return own(out.p);
 }
 
+// ---- a key/value cache in pages (paged.py has the same steps, and the messages for what is refused) ---------------------
+// A plain tensor on device `dev` (-1: any CUDA device, and `dev` is set), null otherwise.
+const at::Tensor* on_device(PyObject* obj, int& dev) {
+    if (!THPVariable_CheckExact(obj)) return nullptr;
+    const at::Tensor& t = THPVariable_Unpack(obj);
+    if (!t.is_cuda()) return nullptr;
+    if (dev < 0) dev = t.device().index();
+    return t.device().index() == dev ? &t : nullptr;
+}
+// int32 with contiguous rows
+const at::Tensor* ints(PyObject* obj, int& dev, int64_t dims) {
+    const at::Tensor* t = on_device(obj, dev);
+    if (t == nullptr || t->scalar_type() != at::kInt || t->dim() != dims || (dims > 0 && t->size(dims - 1) > 1 && t->stride(dims - 1) != 1)) return nullptr;
+    return t;
+}
+int32_t* words(const at::Tensor& t) { return static_cast<int32_t*>(t.data_ptr()); }
+bool whole(PyObject* obj, int64_t* v) {
+    *v = PyLong_CheckExact(obj) ? PyLong_AsLongLong(obj) : -1;
+    if (*v == -1 && PyErr_Occurred()) PyErr_Clear();
+    return *v >= 0;
+}
+cudaStream_t stream_of(int dev) { return c10::cuda::getCurrentCUDAStream((c10::DeviceIndex)dev).stream(); }
+
+struct Tables {
+    const at::Tensor *table, *lens, *free_pages, *count, *change;
+    int64_t B, stride, page;
+    bool read(PyObject* const* args) {
+        int dev = -1;
+        table = ints(args[0], dev, 2);
+        lens = ints(args[1], dev, 1);
+        free_pages = ints(args[2], dev, 1);
+        change = ints(args[4], dev, 1);
+        count = on_device(args[3], dev);
+        if (!table || !lens || !free_pages || !change || !count || count->scalar_type() != at::kInt || count->numel() != 1 || dev != c10::cuda::current_device() ||
+            !whole(args[5], &page) || page > INT32_MAX || free_pages->size(0) > INT32_MAX || table->size(1) > INT32_MAX)
+            return false;
+        B = table->size(0);
+        stride = B > 1 ? table->stride(0) : table->size(1);
+        return B <= INT32_MAX && lens->size(0) == B && change->size(0) == B;
+    }
+    int dev() const { return table->device().index(); }
+};
+
+// paged_reserve(block_table, kv_lens, free_pages, free_count, new_lens, page_size, tokens)
+PyObject* paged_reserve(PyObject*, PyObject* const* args, Py_ssize_t n) {
+    if (n != 7) return PyErr_Format(PyExc_TypeError, "paged_reserve: seven arguments");
+    try {
+        Tables t;
+        int64_t tokens;
+        if (!t.read(args) || !whole(args[6], &tokens) || tokens > INT32_MAX) Py_RETURN_NONE;
+        at::AutoDispatchBelowADInplaceOrView guard;
+        const int64_t B = t.B, sizes[5] = {B + 1, B, tokens, tokens, 1};
+        at::Tensor all = at::empty({2 * B + 2 + 2 * tokens}, t.table->options());
+        int32_t* at = words(all);
+        int32_t *cu = at, *after = cu + B + 1, *positions = after + B, *slots = positions + tokens, *status = slots + tokens;
+        int rc;
+        Py_BEGIN_ALLOW_THREADS
+        rc = hqm_paged_reserve(words(*t.table), t.stride, words(*t.lens), words(*t.free_pages), words(*t.count), words(*t.change), cu, after, positions,
+                               slots, status, (int32_t)B, (int32_t)t.table->size(1), (int32_t)t.page, (int32_t)t.free_pages->size(0), tokens, stream_of(t.dev()));
+        Py_END_ALLOW_THREADS
+        if (rc < 0) Py_RETURN_NONE;
+        PyObject* out = PyTuple_New(5);
+        int64_t from = 0;
+        for (int i = 0; out != nullptr && i < 5; from += sizes[i++]) PyTuple_SET_ITEM(out, i, THPVariable_Wrap(all.narrow(0, from, sizes[i])));
+        return out;
+    } catch (const std::exception& e) {
+        return PyErr_Format(PyExc_RuntimeError, "%s", e.what());
+    }
+}
+
+// paged_truncate(block_table, kv_lens, free_pages, free_count, keep, page_size)
+PyObject* paged_truncate(PyObject*, PyObject* const* args, Py_ssize_t n) {
+    if (n != 6) return PyErr_Format(PyExc_TypeError, "paged_truncate: six arguments");
+    try {
+        Tables t;
+        if (!t.read(args)) Py_RETURN_NONE;
+        at::AutoDispatchBelowADInplaceOrView guard;
+        at::Tensor status = at::empty({1}, t.table->options());
+        int rc;
+        Py_BEGIN_ALLOW_THREADS
+        rc = hqm_paged_truncate(words(*t.table), t.stride, words(*t.lens), words(*t.free_pages), words(*t.count), words(*t.change), words(status), (int32_t)t.B,
+                                (int32_t)t.table->size(1), (int32_t)t.page, (int32_t)t.free_pages->size(0), stream_of(t.dev()));
+        Py_END_ALLOW_THREADS
+        if (rc < 0) Py_RETURN_NONE;
+        return THPVariable_Wrap(std::move(status));
+    } catch (const std::exception& e) {
+        return PyErr_Format(PyExc_RuntimeError, "%s", e.what());
+    }
+}
+
+// A tensor of `dims` dimensions like q in type, device and its last one, whose elements are contiguous.
+const at::Tensor* like(PyObject* obj, const at::Tensor& q, int64_t dims) {
+    int dev = q.device().index();
+    const at::Tensor* t = on_device(obj, dev);
+    if (t == nullptr || t->scalar_type() != q.scalar_type() || t->dim() != dims || t->size(-1) != q.size(-1) || (t->size(-1) > 1 && t->stride(-1) != 1)) return nullptr;
+    return t;
+}
+const at::Tensor* queries(PyObject* obj) {
+    int dev = -1;
+    const at::Tensor* q = on_device(obj, dev);
+    if (q == nullptr || q->dim() != 3 || (q->scalar_type() != at::kBFloat16 && q->scalar_type() != at::kHalf) || dev != c10::cuda::current_device() ||
+        (q->size(2) > 1 && q->stride(2) != 1) || q->size(0) > INT32_MAX)
+        return nullptr;
+    return q;
+}
+// strides of (tokens, heads, head_dim); of a dimension of one, what a contiguous tensor has
+void strides(const at::Tensor& t, int64_t* token, int64_t* head) {
+    *token = t.size(0) > 1 ? t.stride(0) : t.size(1) * t.size(2);
+    *head = t.size(1) > 1 ? t.stride(1) : t.size(2);
+}
+struct Pool {
+    const at::Tensor *k, *v;
+    int64_t pages, heads, page, k_page, v_page;
+    bool read(PyObject* k_obj, PyObject* v_obj, const at::Tensor& q) {
+        k = like(k_obj, q, 4);
+        v = like(v_obj, q, 4);
+        if (!k || !v || k->sizes() != v->sizes()) return false;
+        pages = k->size(0), heads = k->size(1), page = k->size(2);
+        const int64_t D = k->size(3), one = heads * page * D;
+        for (const at::Tensor* t : {k, v})
+            if ((page > 1 && t->stride(2) != D) || (heads > 1 && t->stride(1) != page * D)) return false;
+        k_page = pages > 1 ? k->stride(0) : one;
+        v_page = pages > 1 ? v->stride(0) : one;
+        return pages <= INT32_MAX && page <= INT32_MAX && heads <= INT32_MAX;
+    }
+};
+// `out`, or a new tensor where it is None; false: of another form than q
+bool result_like(PyObject* obj, const at::Tensor& q, at::Tensor* out) {
+    if (obj == Py_None) {
+        *out = at::empty(q.sizes(), q.options());
+        return true;
+    }
+    const at::Tensor* t = like(obj, q, 3);
+    if (t == nullptr || t->sizes() != q.sizes() || !t->is_contiguous()) return false;
+    *out = *t;
+    return true;
+}
+bool real(PyObject* obj, float* v) {
+    const double d = PyFloat_AsDouble(obj);
+    if (d == -1.0 && PyErr_Occurred()) {
+        PyErr_Clear();
+        return false;
+    }
+    *v = (float)d;
+    return true;
+}
+
+// rope_append_paged(q, k, v, k_pages, v_pages, positions, slots, theta, out or None)
+PyObject* rope_append_paged(PyObject*, PyObject* const* args, Py_ssize_t n) {
+    if (n != 9) return PyErr_Format(PyExc_TypeError, "rope_append_paged: nine arguments");
+    try {
+        const at::Tensor* q = queries(args[0]);
+        if (q == nullptr) Py_RETURN_NONE;
+        const at::Tensor *k = like(args[1], *q, 3), *v = like(args[2], *q, 3);
+        Pool pool;
+        int dev = q->device().index();
+        const at::Tensor *positions = ints(args[5], dev, 1), *slots = ints(args[6], dev, 1);
+        const int64_t T = q->size(0);
+        hqm_paged_append a = {};
+        if (!k || !v || !positions || !slots || !pool.read(args[3], args[4], *q) || k->sizes() != v->sizes() || k->size(0) != T || k->size(1) != pool.heads ||
+            positions->size(0) != T || slots->size(0) != T || !real(args[7], &a.rope_theta))
+            Py_RETURN_NONE;
+        at::AutoDispatchBelowADInplaceOrView guard;
+        at::Tensor out;
+        if (!result_like(args[8], *q, &out)) Py_RETURN_NONE;
+        a.q_out = out.data_ptr();
+        a.q = q->const_data_ptr(), a.k = k->const_data_ptr(), a.v = v->const_data_ptr();
+        strides(*q, &a.q_token, &a.q_head);
+        strides(*k, &a.k_token, &a.k_head);
+        strides(*v, &a.v_token, &a.v_head);
+        a.k_pages = pool.k->data_ptr(), a.v_pages = pool.v->data_ptr();
+        a.k_page = pool.k_page, a.v_page = pool.v_page;
+        a.positions = words(*positions), a.slots = words(*slots);
+        a.tokens = T;
+        a.n_heads = (int32_t)q->size(1), a.n_kv_heads = (int32_t)pool.heads, a.head_dim = (int32_t)q->size(2);
+        a.pages = (int32_t)pool.pages, a.page_size = (int32_t)pool.page;
+        a.dtype = q->scalar_type() == at::kHalf;
+        int rc;
+        Py_BEGIN_ALLOW_THREADS
+        rc = hqm_rope_append_paged(&a, stream_of(dev));
+        Py_END_ALLOW_THREADS
+        if (rc < 0) Py_RETURN_NONE;
+        return THPVariable_Wrap(std::move(out));
+    } catch (const std::exception& e) {
+        return PyErr_Format(PyExc_RuntimeError, "%s", e.what());
+    }
+}
+
+// attention(q, k, v, cu_seqlens, max_new, scale or None, out or None[, block_table, kv_lens]): with the last two k and v are pages
+PyObject* attention(PyObject*, PyObject* const* args, Py_ssize_t n) {
+    if (n != 7 && n != 9) return PyErr_Format(PyExc_TypeError, "attention: seven or nine arguments");
+    try {
+        const bool paged = n == 9;
+        const at::Tensor* q = queries(args[0]);
+        if (q == nullptr) Py_RETURN_NONE;
+        int dev = q->device().index();
+        const int64_t T = q->size(0);
+        hqm_attention c = {};
+        const at::Tensor* cu = ints(args[3], dev, 1);
+        int64_t most = 0;
+        if (cu == nullptr || cu->size(0) < 1 || cu->size(0) > INT32_MAX || !whole(args[4], &most) || most > INT32_MAX) Py_RETURN_NONE;
+        c.sequences = (int32_t)(cu->size(0) - 1);
+        if (paged) {
+            Pool pool;
+            const at::Tensor *table = ints(args[7], dev, 2), *lens = ints(args[8], dev, 1);
+            if (!table || !lens || !pool.read(args[1], args[2], *q) || table->size(0) != c.sequences || lens->size(0) != c.sequences || table->size(1) > INT32_MAX)
+                Py_RETURN_NONE;
+            c.k = pool.k->const_data_ptr(), c.v = pool.v->const_data_ptr();
+            c.k_page = pool.k_page, c.v_page = pool.v_page;
+            c.block_table = words(*table);
+            c.table_stride = c.sequences > 1 ? table->stride(0) : table->size(1);
+            c.kv_lens = words(*lens);
+            c.n_kv_heads = (int32_t)pool.heads, c.pages = (int32_t)pool.pages, c.page_size = (int32_t)pool.page;
+            c.max_pages = (int32_t)table->size(1);
+        } else {
+            const at::Tensor *k = like(args[1], *q, 3), *v = like(args[2], *q, 3);
+            if (!k || !v || k->sizes() != v->sizes() || k->size(0) != T) Py_RETURN_NONE;
+            c.k = k->const_data_ptr(), c.v = v->const_data_ptr();
+            strides(*k, &c.k_token, &c.k_head);
+            strides(*v, &c.v_token, &c.v_head);
+            c.n_kv_heads = (int32_t)k->size(1);
+        }
+        c.scale = 1.f / std::sqrt((float)std::max<int64_t>(q->size(2), 1));
+        if (args[5] != Py_None && !real(args[5], &c.scale)) Py_RETURN_NONE;
+        at::AutoDispatchBelowADInplaceOrView guard;
+        at::Tensor out;
+        if (!result_like(args[6], *q, &out)) Py_RETURN_NONE;
+        c.out = out.data_ptr();
+        c.q = q->const_data_ptr();
+        strides(*q, &c.q_token, &c.q_head);
+        c.cu_seqlens = words(*cu);
+        c.tokens = T;
+        c.max_new = (int32_t)most;
+        c.n_heads = (int32_t)q->size(1), c.head_dim = (int32_t)q->size(2);
+        c.dtype = q->scalar_type() == at::kHalf;
+        const size_t bytes = hqm_attention_scratch_bytes(&c);
+        at::Tensor ws = at::empty({(int64_t)bytes}, q->options().dtype(at::kByte));
+        void* at = ws.data_ptr();
+        int rc;
+        Py_BEGIN_ALLOW_THREADS
+        rc = (paged ? hqm_paged_attention : hqm_prompt_attention)(&c, at, bytes, stream_of(dev));
+        Py_END_ALLOW_THREADS
+        if (rc < 0) Py_RETURN_NONE;
+        return THPVariable_Wrap(std::move(out));
+    } catch (const std::exception& e) {
+        return PyErr_Format(PyExc_RuntimeError, "%s", e.what());
+    }
+}
+
 PyObject* setup(PyObject*, PyObject* const* args, Py_ssize_t n) {
     if (n != 2) return PyErr_Format(PyExc_TypeError, "setup(scratch, grow)");
     Py_INCREF(args[0]);
@@ -349,6 +601,10 @@ PyMethodDef methods[] = {
     {"dequantize", (PyCFunction)(void (*)(void))dequantize, METH_FASTCALL, "dequantize(layer, dtype code) -> tensor or None"},
     {"expert", (PyCFunction)(void (*)(void))expert, METH_FASTCALL, "expert(module, x) -> tensor or None"},
     {"expert_addresses", (PyCFunction)(void (*)(void))expert_addresses, METH_FASTCALL, "expert_addresses(experts) -> bytes or None"},
+    {"paged_reserve", (PyCFunction)(void (*)(void))paged_reserve, METH_FASTCALL, "paged_reserve(...) -> five tensors or None"},
+    {"paged_truncate", (PyCFunction)(void (*)(void))paged_truncate, METH_FASTCALL, "paged_truncate(...) -> tensor or None"},
+    {"rope_append_paged", (PyCFunction)(void (*)(void))rope_append_paged, METH_FASTCALL, "rope_append_paged(...) -> tensor or None"},
+    {"attention", (PyCFunction)(void (*)(void))attention, METH_FASTCALL, "attention(...) -> tensor or None"},
     {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_host", "Host path of the quantized layers.", -1, methods, nullptr, nullptr, nullptr, nullptr};
 

@@ -57,13 +57,15 @@ def paged_reserve(block_table: torch.Tensor, kv_lens: torch.Tensor, free_pages: 
     free_pages[: free_count], block_table, kv_lens and free_count are updated in place.  `tokens`: rows of the step (at least
     the sum of new_lens; the rows behind it get position and slot -1).  All or nothing: with a status other than 0 the
     cache is as it was and the step has no tokens."""
+    step = _cabi.host().paged_reserve(block_table, kv_lens, free_pages, free_count, new_lens, page_size, tokens)
+    if step is not None:
+        return PagedStep(*step)
     B, max_pages, stride = _tables(block_table, kv_lens, free_pages, free_count, new_lens, "new_lens")
     if tokens < 0:
         raise ValueError(f"a step of {tokens} tokens")
     dev = block_table.device
-    # one allocation: cu_seqlens, kv_lens, status, positions, slots
-    cu, after, status, positions, slots = torch.empty(2 * B + 2 + 2 * tokens, dtype=torch.int32, device=dev).split(
-        (B + 1, B, 1, tokens, tokens))
+    cu, after, positions, slots, status = torch.empty(2 * B + 2 + 2 * tokens, dtype=torch.int32, device=dev).split(
+        (B + 1, B, tokens, tokens, 1))
     with torch.cuda.device(dev):
         _cabi.check(_cabi.lib().hqm_paged_reserve(
             _cabi.ptr(block_table), stride, _cabi.ptr(kv_lens), _cabi.ptr(free_pages), _cabi.ptr(free_count), _cabi.ptr(new_lens),
@@ -76,6 +78,9 @@ def paged_truncate(block_table: torch.Tensor, kv_lens: torch.Tensor, free_pages:
                    keep: torch.Tensor, page_size: int) -> torch.Tensor:
     """Every sequence keeps its first keep[b] positions, the pages behind them go back on the stack (hqm_paged_truncate).
     Returns the status (1,): 0, or why nothing changed."""
+    status = _cabi.host().paged_truncate(block_table, kv_lens, free_pages, free_count, keep, page_size)
+    if status is not None:
+        return status
     B, max_pages, stride = _tables(block_table, kv_lens, free_pages, free_count, keep, "keep")
     dev = block_table.device
     status = torch.empty(1, dtype=torch.int32, device=dev)
@@ -131,6 +136,9 @@ def rope_append_paged(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, k_pages
     to the pages at `slots` (T,), in one launch (hqm_rope_append_paged).  Returns the rotated q: `out`, which may be q itself, or
     a new tensor.  Tokens with a negative slot are left out (their rows of `out` stay as they were; of a new tensor they are
     not initialised).  No two tokens may have the same slot.  Angles in 64 bits, one rounding."""
+    done = _cabi.host().rope_append_paged(q, k, v, k_pages, v_pages, positions, slots, theta, out)
+    if done is not None:
+        return done
     if q.dim() != 3 or k.dim() != 3 or v.shape != k.shape or q.shape[0] != k.shape[0]:
         raise ValueError(f"q (T, n_heads, head_dim), k and v (T, n_kv_heads, head_dim), not {tuple(q.shape)}, {tuple(k.shape)}, {tuple(v.shape)}")
     code = _heads(q, k=k, v=v, k_pages=k_pages, v_pages=v_pages)
@@ -165,6 +173,9 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     pages already.  New token i of n sees positions 0 .. kv_lens[b] - n + i; a row that sees nothing is 0.  max_new: no sequence
     has more new tokens (1 for a decoding step).  scale: 1 / sqrt(head_dim) unless given.  Rows behind the last sequence are
     left as they were in `out` (of a new tensor they are not initialised)."""
+    done = _cabi.host().attention(q, k_pages, v_pages, cu_seqlens, max_new, scale, out, block_table, kv_lens)
+    if done is not None:
+        return done
     if q.dim() != 3:
         raise ValueError(f"q is (T, n_heads, head_dim), not {tuple(q.shape)}")
     code = _heads(q, k_pages=k_pages, v_pages=v_pages)
@@ -189,6 +200,9 @@ def prompt_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqle
     """Causal attention over whole prompts, packed one behind the other (hqm_prompt_attention): q (T, n_heads, head_dim), k and v
     (T, n_kv_heads, head_dim), sequence b's rows are cu_seqlens[b] .. cu_seqlens[b + 1] - 1.  max_len: no prompt is longer (T
     unless given).  scale and out as for paged_attention."""
+    done = _cabi.host().attention(q, k, v, cu_seqlens, q.shape[0] if max_len is None else max_len, scale, out)
+    if done is not None:
+        return done
     if q.dim() != 3 or k.dim() != 3 or v.shape != k.shape or q.shape[0] != k.shape[0]:
         raise ValueError(f"q (T, n_heads, head_dim), k and v (T, n_kv_heads, head_dim), not {tuple(q.shape)}, {tuple(k.shape)}, {tuple(v.shape)}")
     code = _heads(q, k=k, v=v)
