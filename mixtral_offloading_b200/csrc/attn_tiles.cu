@@ -93,6 +93,12 @@ __device__ __forceinline__ void copy_box(uint32_t dst, const CUtensorMap* map, i
 __device__ __forceinline__ void fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
 
+// A lane's row lies in lines of its own, so that the stores of a warp take a cycle per lane and instruction: as wide as they come.
+__device__ __forceinline__ void store_32_bytes(void* at, const uint32_t* v) {
+    asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(at), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]),
+                 "r"(v[6]), "r"(v[7]) : "memory");
+}
+
 // Two floats for the packed instructions.
 typedef unsigned long long Pair;
 __device__ __forceinline__ Pair pair(float lo, float hi) {
@@ -335,19 +341,13 @@ __global__ void __launch_bounds__(THREADS, 1) attn_tiles_kernel(const __grid_con
                 loads_done(o);
                 if (!valid) continue;
                 if (whole) {
-                    uint4* dst = reinterpret_cast<uint4*>(a.out + row * D + c);
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        uint32_t v[4];
-#pragma unroll
-                        for (int e = 0; e < 4; ++e)
-                            v[e] = pack2(__uint_as_float(o[8 * i + 2 * e]) * inv, __uint_as_float(o[8 * i + 2 * e + 1]) * inv, F16);
-                        dst[i] = make_uint4(v[0], v[1], v[2], v[3]);
-                    }
+                    for (int i = 0; i < 16; ++i) o[i] = pack2(__uint_as_float(o[2 * i]) * inv, __uint_as_float(o[2 * i + 1]) * inv, F16);
+                    store_32_bytes(a.out + row * D + c, o);
+                    store_32_bytes(a.out + row * D + c + 16, o + 8);
                 } else {
-                    uint4* dst = reinterpret_cast<uint4*>(piece + pr * D + c);
 #pragma unroll
-                    for (int i = 0; i < 8; ++i) dst[i] = make_uint4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
+                    for (int i = 0; i < 32; i += 8) store_32_bytes(piece + pr * D + c + i, o + i);
                 }
             }
             fence_before();
