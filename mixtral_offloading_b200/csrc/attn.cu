@@ -23,15 +23,31 @@ int sm_count() {
     return n;
 }
 
-// Boxes of 64 x y x z x w elements, 128-byte swizzle; strides in elements.
-bool encode(CUtensorMap* to, const void* at, const cuuint64_t (&dims)[4], const int64_t (&strides)[3], int y, int z, int w, bool f16) {
+// Strides in elements.  Boxes start at 64 columns, 128-byte swizzle.
+bool encode(CUtensorMap* to, const void* at, int rank, const cuuint64_t* dims, const int64_t* strides, const cuuint32_t* box, bool f16) {
     const EncodeTiledFn enc = (EncodeTiledFn)tma_encode_entry();
     if (!enc) return false;
-    const cuuint32_t ones[4] = {1, 1, 1, 1}, box[4] = {64, (cuuint32_t)y, (cuuint32_t)z, (cuuint32_t)w};
-    const cuuint64_t bytes[3] = {(cuuint64_t)strides[0] * 2, (cuuint64_t)strides[1] * 2, (cuuint64_t)strides[2] * 2};
-    return enc(to, f16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, const_cast<void*>(at), dims, bytes, box, ones,
+    const cuuint32_t ones[5] = {1, 1, 1, 1, 1};
+    cuuint64_t bytes[4];
+    for (int i = 0; i < rank - 1; ++i) bytes[i] = (cuuint64_t)strides[i] * 2;
+    return enc(to, f16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, rank, const_cast<void*>(at), dims, bytes, box, ones,
                CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
                CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+// Keys or values: `rows` positions of one head of one page (packed: of the one page that all of them are).  `across`: 64 columns
+// after another in one box; else one box brings 64 columns.
+bool encode_kv(CUtensorMap* to, const void* at, int D, int rows, cuuint64_t positions, cuuint64_t heads, cuuint64_t pages, int64_t position, int64_t head,
+               int64_t page, bool across, bool f16) {
+    if (across) {
+        const cuuint64_t dims[5] = {64, positions, (cuuint64_t)D / 64, heads, pages};
+        const int64_t strides[4] = {position, 64, head, page};
+        const cuuint32_t box[5] = {64, (cuuint32_t)rows, (cuuint32_t)D / 64, 1, 1};
+        return encode(to, at, 5, dims, strides, box, f16);
+    }
+    const cuuint64_t dims[4] = {(cuuint64_t)D, positions, heads, pages};
+    const int64_t strides[3] = {position, head, page};
+    const cuuint32_t box[4] = {64, (cuuint32_t)rows, 1, 1};
+    return encode(to, at, 4, dims, strides, box, f16);
 }
 
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
@@ -63,9 +79,19 @@ int check(const hqm_attention* c, bool paged, const char* what) {
     return HQM_OK;
 }
 
-// Whether a unit of attn_few.cu holds all new tokens of any sequence.
-bool few_rows(const hqm_attention* c) { return (int64_t)c->max_new * (c->n_heads / c->n_kv_heads) <= FEW_TILE; }
-int rows_of_piece(const hqm_attention* c) { return few_rows(c) ? FEW_TILE : TILE_ROWS; }
+// Which kernels a call takes: attn_few.cu where its unit holds all new tokens of any sequence, else attn_tiles.cu.  Where the
+// sequences beside the longest have few rows on average, both: those that fit a unit of attn_few.cu run there, at the
+// rate of the memory, and do not fill a tile of 128 rows with four.
+struct Kernels {
+    bool few, tiles;
+    static Kernels of(const hqm_attention* c, bool paged) {
+        const int64_t group = c->n_heads / c->n_kv_heads, most = c->max_new < c->tokens ? c->max_new : c->tokens;
+        if (most * group <= FEW_TILE) return {true, false};
+        const bool mixed = paged && group <= FEW_TILE && (c->tokens - most) * group <= (int64_t)MIXED_ROWS * (c->sequences - 1);
+        return {mixed && c->sequences > 1, true};
+    }
+};
+size_t launch_bytes(int ctas, int rows, int D) { return record_bytes(ctas) + (piece_bytes(ctas, rows, D) + 255) / 256 * 256; }
 
 int run(const hqm_attention* c, bool paged, const char* what, void* scratch, size_t scratch_bytes, void* stream) {
     if (int rc = check(c, paged, what)) return rc;
@@ -98,33 +124,50 @@ int run(const hqm_attention* c, bool paged, const char* what, void* scratch, siz
     if (paged)
         while ((1 << a.page_shift) < c->page_size) ++a.page_shift;
     a.scale_log2 = (float)((double)c->scale * 1.4426950408889634);
-    a.records = (int32_t*)scratch;
-    a.pieces = (float*)((uint8_t*)scratch + record_bytes(ctas));
-    a.piece_rows = rows_of_piece(c);
-    CUtensorMap qm, km, vm;
-    const bool few = few_rows(c);
-    const int keys = few ? FEW_KEYS : TILE_KEYS, box = paged && c->page_size < keys ? c->page_size : keys;
-    bool ok;
-    if (paged) {
-        const cuuint64_t dims[4] = {(cuuint64_t)D, (cuuint64_t)c->page_size, (cuuint64_t)c->n_kv_heads, (cuuint64_t)c->pages};
-        const int64_t head = (int64_t)c->page_size * D;
-        ok = encode(&km, c->k, dims, {(int64_t)D, head, c->k_page}, box, 1, 1, f16) && encode(&vm, c->v, dims, {(int64_t)D, head, c->v_page}, box, 1, 1, f16);
-    } else {
-        const cuuint64_t dims[4] = {(cuuint64_t)D, (cuuint64_t)c->tokens, (cuuint64_t)c->n_kv_heads, 1};
-        ok = encode(&km, c->k, dims, {c->k_token, c->k_head, c->k_token * c->tokens}, box, 1, 1, f16) && encode(&vm, c->v, dims, {c->v_token, c->v_head, c->v_token * c->tokens}, box, 1, 1, f16);
-    }
-    if (ok && !few) {
-        // row = token * group + head: a box of all heads of a group and as many tokens as a tile holds
-        const cuuint64_t dims[4] = {(cuuint64_t)D, (cuuint64_t)a.group, (cuuint64_t)c->n_kv_heads, (cuuint64_t)c->tokens};
-        ok = encode(&qm, c->q, dims, {c->q_head, c->q_head * a.group, c->q_token}, a.group, 1, 128 / a.group, f16);
-    }
-    if (!ok) {
+    Args few = a, tiles = a;
+    uint8_t* at = (uint8_t*)scratch;
+    auto place = [&](Args& to, int rows) {
+        to.records = (int32_t*)at;
+        to.pieces = (float*)(at + record_bytes(ctas));
+        to.piece_rows = rows;
+        at += launch_bytes(ctas, rows, D);
+    };
+    const Kernels k = Kernels::of(c, paged);
+    few.rows_above = tiles.rows_above = 0;
+    few.rows_upto = tiles.rows_upto = INT32_MAX;
+    if (k.few && k.tiles) few.rows_upto = tiles.rows_above = FEW_TILE;
+    // keys and values: rows of a box, and whether it brings all columns
+    auto maps = [&](CUtensorMap* km, CUtensorMap* vm, int keys, bool across) {
+        if (paged) {
+            const int rows = c->page_size < keys ? c->page_size : keys;
+            const int64_t head = (int64_t)c->page_size * D;
+            return encode_kv(km, c->k, D, rows, c->page_size, c->n_kv_heads, c->pages, D, head, c->k_page, across, f16) &&
+                   encode_kv(vm, c->v, D, rows, c->page_size, c->n_kv_heads, c->pages, D, head, c->v_page, across, f16);
+        }
+        return encode_kv(km, c->k, D, keys, c->tokens, c->n_kv_heads, 1, c->k_token, c->k_head, c->k_token * c->tokens, across, f16) &&
+               encode_kv(vm, c->v, D, keys, c->tokens, c->n_kv_heads, 1, c->v_token, c->v_head, c->v_token * c->tokens, across, f16);
+    };
+    auto no_maps = [&]() {
         set_error("%s: the driver does not encode the tensor maps", what);
         return HQM_ERR_CUDA;
-    }
+    };
     const cudaStream_t st = (cudaStream_t)stream;
-    if (int rc = few ? launch_few(a, km, vm, ctas, D, f16, st) : launch_tiles(a, qm, km, vm, ctas, D, f16, st)) return rc;
-    return launch_join(a, ctas, D, f16, st);
+    CUtensorMap qm, km, vm;
+    if (k.tiles) {
+        place(tiles, TILE_ROWS);
+        // row = token * group + head: a box of all heads of a group and as many tokens as a tile holds
+        const cuuint64_t dims[4] = {(cuuint64_t)D, (cuuint64_t)a.group, (cuuint64_t)c->n_kv_heads, (cuuint64_t)c->tokens};
+        const int64_t strides[3] = {c->q_head, c->q_head * a.group, c->q_token};
+        const cuuint32_t box[4] = {64, (cuuint32_t)a.group, 1, 128u / a.group};
+        if (!maps(&km, &vm, TILE_KEYS, false) || !encode(&qm, c->q, 4, dims, strides, box, f16)) return no_maps();
+        if (int rc = launch_tiles(tiles, qm, km, vm, ctas, D, f16, st)) return rc;
+    }
+    if (k.few) {
+        place(few, FEW_TILE);
+        if (!maps(&km, &vm, FEW_KEYS, true)) return no_maps();
+        if (int rc = launch_few(few, km, vm, ctas, D, f16, st)) return rc;
+    }
+    return launch_join(k.tiles ? tiles : few, k.tiles && k.few ? &few : nullptr, ctas, D, f16, st);
 }
 
 }  // namespace
@@ -135,9 +178,10 @@ extern "C" {
 
 size_t hqm_attention_scratch_bytes(const hqm_attention* c) {
     using namespace hqm::attn;
-    if (!c) return 0;
+    if (!c || c->n_kv_heads <= 0 || c->n_heads < c->n_kv_heads) return 0;
     const int ctas = sm_count() > 0 ? sm_count() : 148;
-    return record_bytes(ctas) + piece_bytes(ctas, rows_of_piece(c), c->head_dim);
+    const Kernels k = Kernels::of(c, c->block_table != nullptr);
+    return (k.tiles ? launch_bytes(ctas, TILE_ROWS, c->head_dim) : 0) + (k.few ? launch_bytes(ctas, FEW_TILE, c->head_dim) : 0);
 }
 int hqm_paged_attention(const hqm_attention* call, void* scratch, size_t scratch_bytes, void* stream) {
     return hqm::attn::run(call, true, "paged_attention", scratch, scratch_bytes, stream);

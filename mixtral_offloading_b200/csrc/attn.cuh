@@ -33,6 +33,7 @@ struct Args {
     float* pieces;                 // two per CTA
     int32_t* records;              // of CTA c: the unit that starts in c and is cut behind it (RECORD words)
     int piece_rows;                // rows of a piece
+    int rows_above, rows_upto;     // the launch is about sequences with that many rows per key/value head
 };
 constexpr int RECORD = 8;          // q0, tokens, head, first token, CTAs (0: none), 3 unused
 
@@ -92,7 +93,8 @@ __device__ __forceinline__ Seq load_seq(const Args& a, int b, const Cut& c) {
     s.per = c.per;
     s.block = c.block;
     s.extra = c.extra;
-    s.tiles = (s.n + c.per - 1) / c.per;
+    const int64_t rows = (int64_t)s.n * a.group;
+    s.tiles = rows > a.rows_above && rows <= a.rows_upto ? (s.n + c.per - 1) / c.per : 0;
     return s;
 }
 
@@ -230,8 +232,8 @@ __device__ __forceinline__ float ex2(float x) {
     return r;
 }
 
-// Adds the pieces of the units that a cut goes through (attn_few.cu).
-int launch_join(const Args& a, int ctas, int D, bool f16, cudaStream_t st);
+// Adds the pieces of the units that a cut goes through, of one launch or of two (attn_few.cu).
+int launch_join(const Args& a, const Args* more, int ctas, int D, bool f16, cudaStream_t st);
 // attn_few.cu: up to FEW_TILE rows per key/value head.
 int launch_few(const Args& a, const CUtensorMap& km, const CUtensorMap& vm, int ctas, int D, bool f16, cudaStream_t st);
 
@@ -242,6 +244,7 @@ constexpr int FEW_TILE = 16;       // rows of a unit of attn_few.cu
 constexpr int FEW_KEYS = 64;       // positions of a block there
 constexpr int TILE_ROWS = 256;     // rows of a unit of attn_tiles.cu
 constexpr int TILE_KEYS = 128;      // positions of a block there
+constexpr int MIXED_ROWS = 64;     // see attn.cu
 constexpr int MAX_GROUP = 128;     // query heads per key/value head: the rows of a tile
 
 }  // namespace attn

@@ -19,23 +19,24 @@ namespace {
 constexpr int CONSUMERS = 8;
 constexpr int THREADS = 32 * (CONSUMERS + 1);
 constexpr int STAGES = 4;
+static_assert(STAGES % 2 == 0, "the halves of the warps take turns: a buffer belongs to one half, or that one would skip every other phase");
 constexpr int UNIT_EXTRA = 1;          // what a unit costs beside its blocks, in blocks
 
 template <int D>
 struct Shared {
     static constexpr int HALVES = D / 64;
-    static constexpr int TILE = FEW_KEYS * 128;                   // 64 positions x 64 columns, 128-byte swizzle
-    static constexpr int STAGE = 2 * HALVES * TILE;
-    alignas(1024) unsigned char ring[STAGES][STAGE];              // K halves, V halves
+    static constexpr int TILE = FEW_KEYS * 128 * HALVES;          // 64 positions: boxes of [64 columns][rows of a box][128 bytes], 128-byte swizzle
+    alignas(1024) unsigned char ring[STAGES][2][TILE];            // K, V
     float sums[CONSUMERS][FEW_TILE][D];
     float top[CONSUMERS][FEW_TILE], total[CONSUMERS][FEW_TILE];
     uint64_t full[STAGES], empty[STAGES];
     Run run;
 };
 
-__device__ __forceinline__ void copy_box(uint32_t dst, const CUtensorMap* map, int x, int row, int head, int page, uint32_t bar) {
-    asm volatile("cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];"
-                 ::"r"(dst), "l"(map), "r"(x), "r"(row), "r"(head), "r"(page), "r"(bar)
+// All columns of `rows` positions: [64 columns][rows][128 bytes].
+__device__ __forceinline__ void copy_box(uint32_t dst, const CUtensorMap* map, int row, int head, int page, uint32_t bar) {
+    asm volatile("cp.async.bulk.tensor.5d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %2, %4, %5}], [%6];"
+                 ::"r"(dst), "l"(map), "r"(0), "r"(row), "r"(head), "r"(page), "r"(bar)
                  : "memory");
 }
 __device__ __forceinline__ void expect(uint32_t bar, uint32_t bytes) {
@@ -83,33 +84,35 @@ __global__ void __launch_bounds__(THREADS, 1) attn_few_kernel(const __grid_const
     const Run run = sh.run;
     Walk w(a, run, how);
     bool ok = true;
+    const int rows = a.table ? min(1 << a.page_shift, FEW_KEYS) : FEW_KEYS, boxes = FEW_KEYS / rows;       // of a box, per block
     if (warp == CONSUMERS) {
-        // ---- the copies: lane i brings box i of a stage ----
-        const int page_rows = min(1 << a.page_shift, FEW_KEYS);
-        const int rows = a.table ? page_rows : FEW_KEYS;                   // of a box
-        const int boxes = FEW_KEYS / rows;                                 // per 64 columns
+        // ---- the copies: lane i brings box i of a stage, K and V ----
         uint32_t at = 0;
         while (w.next() && ok) {
-            const int64_t trow = (int64_t)w.b * a.table_stride;
-            for (int j = w.j0; j < w.j1 && ok; ++j, ++at) {
+            const int32_t* table = a.table + (int64_t)w.b * a.table_stride;
+            // of block j; read one block ahead of the copies
+            auto place = [&](int j, int& row, int& page) {
+                const int key = j * FEW_KEYS + lane * rows;
+                row = w.s.q0 + key;
+                page = 0;
+                if (!a.table || lane >= boxes || key >= w.s.kv) return;
+                page = min((uint32_t)table[key >> a.page_shift], (uint32_t)a.n_pages);           // outside the pool: zeros
+                row = key & ((1 << a.page_shift) - 1);
+            };
+            int row, page, next_row = 0, next_page = 0;
+            place(w.j0, row, page);
+            for (int j = w.j0; j < w.j1 && ok; ++j, ++at, row = next_row, page = next_page) {
+                if (j + 1 < w.j1) place(j + 1, next_row, next_page);
                 const int stage = at % STAGES;
                 if (at >= STAGES) ok = __all_sync(0xffffffffu, tc::mbar_wait(&sh.empty[stage], (at / STAGES - 1) & 1));
                 if (!ok) break;
-                const int key0 = j * FEW_KEYS;
-                const int live = min(boxes, (max(w.s.kv - key0, 0) + rows - 1) / rows);      // boxes that hold positions of the sequence
+                const int live = min(boxes, (max(w.s.kv - j * FEW_KEYS, 0) + rows - 1) / rows);  // boxes that hold positions of the sequence
                 const uint32_t bar = tc::smem_u32(&sh.full[stage]);
                 if (lane == 0) expect(bar, (uint32_t)live * rows * 128 * S::HALVES * 2);
                 __syncwarp();
-                for (int i = lane; i < live * 2 * S::HALVES; i += 32) {
-                    const int box = i % live, what = i / live;             // K halves, then V halves
-                    const int key = key0 + box * rows;
-                    int row = w.s.q0 + key, page = 0;
-                    if (a.table) {
-                        page = min((uint32_t)a.table[trow + (key >> a.page_shift)], (uint32_t)a.n_pages);      // outside the pool: zeros
-                        row = key & ((1 << a.page_shift) - 1);
-                    }
-                    copy_box(tc::smem_u32(sh.ring[stage] + what * S::TILE + box * rows * 128), what < S::HALVES ? &km : &vm,
-                             (what % S::HALVES) * 64, row, w.h, page, bar);
+                if (lane < live) {
+                    copy_box(tc::smem_u32(sh.ring[stage][0] + lane * rows * 128 * S::HALVES), &km, row, w.h, page, bar);
+                    copy_box(tc::smem_u32(sh.ring[stage][1] + lane * rows * 128 * S::HALVES), &vm, row, w.h, page, bar);
                 }
                 __syncwarp();
             }
@@ -122,6 +125,11 @@ __global__ void __launch_bounds__(THREADS, 1) attn_few_kernel(const __grid_const
     // ---- the products ----
     const int half = warp >> 2, strip = (warp & 3) * 16;                   // stages of this half, positions within a stage
     const int r0 = lane >> 2, c0 = (lane & 3) * 2;                         // rows r0 and r0 + 8, columns c0, c0 + 1 of an 8-wide tile
+    // where position `key` of a stage lies, its first 64 columns; the next 64 are `across` bytes further on
+    auto key_at = [&](int key) { return (uint32_t)(((key & ~(rows - 1)) * S::HALVES + (key & (rows - 1))) * 128); };
+    const int across = rows * 128;
+    const int krow = strip + (lane & 7) + ((lane >> 4) << 3), kch = (lane >> 3) & 1, vrow = strip + (lane & 15), vch = lane >> 4;
+    const uint32_t k_off = key_at(krow), v_off = key_at(vrow);
     uint32_t at = 0;
     bool cut = false;
     while (w.next()) {
@@ -147,16 +155,15 @@ __global__ void __launch_bounds__(THREADS, 1) attn_few_kernel(const __grid_const
             if ((int)(at & 1) != half) continue;
             const int stage = at % STAGES;
             ok = ok && __all_sync(0xffffffffu, tc::mbar_wait(&sh.full[stage], (at / STAGES) & 1));
-            const uint32_t kt = tc::smem_u32(sh.ring[stage]), vt = kt + S::HALVES * S::TILE;
+            const uint32_t kt = tc::smem_u32(sh.ring[stage][0]) + k_off, vt = tc::smem_u32(sh.ring[stage][1]) + v_off;
             const int key0 = j * FEW_KEYS + strip;
             if (key0 < w.s.kv) {
                 float s[2][4] = {};
-                const int krow = strip + (lane & 7) + ((lane >> 4) << 3), kch = (lane >> 3) & 1;
 #pragma unroll
                 for (int k = 0; k < D / 16; ++k) {
                     uint32_t b[4];
                     const int ch = (2 * k + kch) & 7;
-                    ldsm(b, kt + (k >> 2) * S::TILE + krow * 128 + ((ch ^ (krow & 7)) << 4));
+                    ldsm(b, kt + (k >> 2) * across + ((ch ^ (krow & 7)) << 4));
                     mma<F16>(s[0], qf[k], b[0], b[1]);
                     mma<F16>(s[1], qf[k], b[2], b[3]);
                 }
@@ -197,7 +204,6 @@ __global__ void __launch_bounds__(THREADS, 1) attn_few_kernel(const __grid_const
                     }
                 const uint32_t p[4] = {pack2(s[0][0], s[0][1], F16), pack2(s[0][2], s[0][3], F16), pack2(s[1][0], s[1][1], F16),
                                        pack2(s[1][2], s[1][3], F16)};
-                const int vrow = strip + (lane & 15), vch = lane >> 4;
                 // what lies behind the sequence is anything, also NaN, which no weight of zero takes away
                 const int past = key0 + 16 - w.s.kv;
                 const int k0 = key0 + c0;
@@ -207,7 +213,7 @@ __global__ void __launch_bounds__(THREADS, 1) attn_few_kernel(const __grid_const
                 for (int d = 0; d < D / 16; ++d) {
                     uint32_t b[4];
                     const int ch = (2 * d + vch) & 7;
-                    ldsm_t(b, vt + (d >> 2) * S::TILE + vrow * 128 + ((ch ^ (vrow & 7)) << 4));
+                    ldsm_t(b, vt + (d >> 2) * across + ((ch ^ (vrow & 7)) << 4));
                     mma<F16>(o[2 * d], p, b[0] & m0, b[1] & m1);
                     mma<F16>(o[2 * d + 1], p, b[2] & m0, b[3] & m1);
                 }
@@ -271,12 +277,13 @@ __global__ void __launch_bounds__(THREADS, 1) attn_few_kernel(const __grid_const
     if (!ok && lane == 0 && error_flag) atomicExch(error_flag, 1);
 }
 
-// CTA (c, y): rows y, y + gridDim.y, ... of the unit whose first piece is CTA c's, a warp per row.
+// CTA (c, y): rows y, y + gridDim.y, ... of the unit whose first piece is CTA c's (of launch `one`, then of `two`), a warp per row.
 template <int D, bool F16>
-__global__ void __launch_bounds__(128) attn_join_kernel(const __grid_constant__ Args a) {
+__global__ void __launch_bounds__(128) attn_join_kernel(const __grid_constant__ Args one, const __grid_constant__ Args two, int ctas_of_one) {
     grid_launch_dependents();
     grid_dependency_wait();
-    const int c = blockIdx.x, lane = threadIdx.x & 31;
+    const Args& a = blockIdx.x < ctas_of_one ? one : two;
+    const int c = blockIdx.x < ctas_of_one ? blockIdx.x : blockIdx.x - ctas_of_one, lane = threadIdx.x & 31;
     const int32_t* rec = a.records + (int64_t)c * RECORD;
     const int ctas = __ldcg(rec + 4);
     if (ctas == 0) return;
@@ -331,10 +338,12 @@ int launch_few(const Args& a, const CUtensorMap& km, const CUtensorMap& vm, int 
     return f16 ? few_launch<64, true>(a, km, vm, ctas, st) : few_launch<64, false>(a, km, vm, ctas, st);
 }
 
-int launch_join(const Args& a, int ctas, int D, bool f16, cudaStream_t st) {
-    const dim3 grid(ctas, (a.piece_rows + 15) / 16 < 4 ? 4 : (a.piece_rows + 15) / 16);
-    if (D == 128) HQM_CUDA(launch_overlapped(f16 ? attn_join_kernel<128, true> : attn_join_kernel<128, false>, grid, 128, 0, st, a));
-    else HQM_CUDA(launch_overlapped(f16 ? attn_join_kernel<64, true> : attn_join_kernel<64, false>, grid, 128, 0, st, a));
+int launch_join(const Args& a, const Args* more, int ctas, int D, bool f16, cudaStream_t st) {
+    const int rows = more && more->piece_rows > a.piece_rows ? more->piece_rows : a.piece_rows;
+    const dim3 grid(more ? 2 * ctas : ctas, (rows + 15) / 16 < 4 ? 4 : (rows + 15) / 16);
+    const Args& b = more ? *more : a;
+    if (D == 128) HQM_CUDA(launch_overlapped(f16 ? attn_join_kernel<128, true> : attn_join_kernel<128, false>, grid, 128, 0, st, a, b, ctas));
+    else HQM_CUDA(launch_overlapped(f16 ? attn_join_kernel<64, true> : attn_join_kernel<64, false>, grid, 128, 0, st, a, b, ctas));
     HQM_LAUNCH_CHECK();
     return HQM_OK;
 }

@@ -4,28 +4,25 @@
 // table[b][0 .. ceil(len_b / P) - 1].  n_b new tokens need ceil((len_b + n_b) / P) - ceil(len_b / P) pages more; with F_b the sum of
 // what the sequences before b need, page i of them is free[count - 1 - (F_b + i)], and new token t of all has position
 // len_b + t - cu_b and the slot (page of its position) * P + position % P.  All of it is two prefix sums over the sequences and a
-// search per page and token, so a token's page is known without waiting for the table to be written.  Bound by latency: one
-// launch, every CTA of a cluster forms the sums for itself, the cluster's barrier lies between the last read of the state and
-// its first write.
+// search per page and token.  Bound by latency: one CTA, which takes a token's page off the stack without waiting for the
+// table; positions and slots of more than 4096 tokens are left to a second launch of as many CTAs as it takes (102000 tokens of 256
+// sequences: 27 us in one launch of eight CTAs, 9 so).
 //
 // Append.  turn = position * theta^(-2 d / D) / 2 pi in 64 bits (a position of 10^5 leaves 32 bits with 10^-2 of an angle), its
 // fraction in 32; (a, b) -> (a cos - b sin, b cos + a sin) in fp32, rounded once.  Bound by bytes: q in and out, k and v into
 // their pages, sixteen at a time.
-#include <cooperative_groups.h>
 #include <math.h>
 
 #include "common.cuh"
 #include "kernels.cuh"
 #include "shared_limit.h"
 
-namespace cg = cooperative_groups;
-
 namespace hqm {
 namespace {
 
 constexpr int TABLE_THREADS = 512;
-constexpr int TABLE_CLUSTER = 8;             // CTAs from TABLE_ALONE tokens on
 constexpr int64_t TABLE_ALONE = 4096;
+constexpr int MAP_THREADS = 256, MAP_TOKENS = 4 * MAP_THREADS;
 constexpr int MAX_SEQUENCES = 16384;         // three words of shared memory each
 
 struct Tables {
@@ -36,6 +33,7 @@ struct Tables {
     int32_t *cu, *after, *positions, *slots, *status;
     int B, max_pages, page, capacity;        // capacity: of free_pages
     int64_t tokens;
+    int maps;                                // positions and slots as well
 };
 
 __device__ __forceinline__ int64_t shift_up(int64_t v, int o) { return __shfl_up_sync(0xffffffffu, v, o); }
@@ -60,7 +58,6 @@ __global__ void __launch_bounds__(TABLE_THREADS) tables_kernel(const __grid_cons
     int32_t* s_len = words + 2 * (p.B + 1);
     __shared__ int64_t s_sum[2][TABLE_THREADS / 32];
     __shared__ int s_bad;
-    cg::cluster_group cluster = cg::this_cluster();
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     if (threadIdx.x == 0) s_bad = 0;
     grid_launch_dependents();
@@ -116,8 +113,9 @@ __global__ void __launch_bounds__(TABLE_THREADS) tables_kernel(const __grid_cons
     else if (count < 0 || count > p.capacity || (!TAKE && base[1] > p.capacity - count)) status = -3;
     else if (TAKE && base[1] > count) status = (int)(base[1] - count < INT32_MAX ? base[1] - count : INT32_MAX);
     const int n_tokens = status == 0 ? (int)base[0] : 0, n_pages = status == 0 ? (int)base[1] : 0;
-    cluster.sync();
-    const int tid = cluster.block_rank() * TABLE_THREADS + threadIdx.x, all = cluster.num_blocks() * TABLE_THREADS;
+    const int tid = threadIdx.x;
+    constexpr int all = TABLE_THREADS;
+    __syncthreads();                         // the last read of lengths and count lies in front, their first write behind
     const int top = TAKE ? count - 1 : count + n_pages - 1;
     for (int i = tid; i < n_pages; i += all) {
         const int b = range_of(s_pg, p.B, i);
@@ -127,7 +125,7 @@ __global__ void __launch_bounds__(TABLE_THREADS) tables_kernel(const __grid_cons
         else p.free_pages[top - i] = *entry;
     }
     if (TAKE) {
-        for (int64_t t = tid; t < p.tokens; t += all) {
+        for (int64_t t = tid; p.maps && t < p.tokens; t += all) {
             int position = -1, slot = -1;
             if (t < n_tokens) {
                 const int b = range_of(s_cu, p.B, (int)t);
@@ -153,16 +151,52 @@ __global__ void __launch_bounds__(TABLE_THREADS) tables_kernel(const __grid_cons
     }
 }
 
-int launch_tables(const Tables& p, bool take, cudaStream_t st) {
-    static SharedLimits limits[2];
-    const size_t bytes = (size_t)(3 * p.B + 2) * sizeof(int32_t);
-    const int cluster = p.tokens > TABLE_ALONE ? TABLE_CLUSTER : 1;
+// Positions and slots from the offsets, lengths and table that tables_kernel leaves: MAP_TOKENS tokens per CTA.
+__global__ void __launch_bounds__(MAP_THREADS) maps_kernel(const __grid_constant__ Tables p) {
+    extern __shared__ int32_t words[];
+    __shared__ int s_first, s_last;
+    grid_launch_dependents();
+    grid_dependency_wait();
+    const int64_t t0 = (int64_t)blockIdx.x * MAP_TOKENS;
+    const int n_tokens = p.cu[p.B];
+    // the sequences of this CTA's tokens: their offsets in shared memory
+    if (threadIdx.x < 2) {
+        const int64_t t = threadIdx.x == 0 ? t0 : t0 + MAP_TOKENS - 1;
+        const int at = range_of(p.cu, p.B, (int)(t < n_tokens - 1 ? t : (n_tokens > 0 ? n_tokens - 1 : 0)));
+        (threadIdx.x == 0 ? s_first : s_last) = at;
+    }
+    __syncthreads();
+    const int first = s_first, count = p.B > 0 ? s_last - first + 1 : 0;
+    for (int i = threadIdx.x; i <= count; i += MAP_THREADS) words[i] = p.cu[first + i];
+    __syncthreads();
+#pragma unroll
+    for (int k = 0; k < MAP_TOKENS / MAP_THREADS; ++k) {
+        const int64_t t = t0 + k * MAP_THREADS + threadIdx.x;
+        if (t >= p.tokens) return;
+        int position = -1, slot = -1;
+        if (t < n_tokens) {
+            const int i = range_of(words, count, (int)t), b = first + i;
+            position = p.after[b] - (words[i + 1] - (int)t);
+            slot = (int)((int64_t)p.table[(int64_t)b * p.stride + position / p.page] * p.page + position % p.page);
+        }
+        p.positions[t] = position;
+        p.slots[t] = slot;
+    }
+}
+
+int launch_tables(Tables p, bool take, cudaStream_t st) {
+    static SharedLimits limits[3];
+    const size_t bytes = (size_t)(3 * p.B + 2) * sizeof(int32_t), map_bytes = (size_t)(p.B + 1) * sizeof(int32_t);
     void (*kernel)(const Tables) = take ? tables_kernel<true> : tables_kernel<false>;
-    if (bytes > 40 * 1024 && !allow_shared(kernel, limits[take], bytes)) {
+    p.maps = p.tokens <= TABLE_ALONE;
+    if ((bytes > 40 * 1024 && !allow_shared(kernel, limits[take], bytes)) || (map_bytes > 40 * 1024 && !allow_shared(maps_kernel, limits[2], map_bytes))) {
         set_error("paged tables: %d sequences want %zu bytes of shared memory", p.B, bytes);
         return HQM_ERR_CUDA;
     }
-    HQM_CUDA(launch_overlapped_cluster(kernel, cluster, TABLE_THREADS, bytes, cluster, st, p));
+    HQM_CUDA(launch_overlapped(kernel, 1, TABLE_THREADS, bytes, st, p));
+    HQM_LAUNCH_CHECK();
+    if (p.maps) return HQM_OK;
+    HQM_CUDA(launch_overlapped(maps_kernel, (int)((p.tokens + MAP_TOKENS - 1) / MAP_TOKENS), MAP_THREADS, map_bytes, st, p));
     HQM_LAUNCH_CHECK();
     return HQM_OK;
 }
@@ -221,6 +255,28 @@ __global__ void __launch_bounds__(APPEND_THREADS) rope_append_paged_kernel(const
         if (threadIdx.x == 0 && error_flag) atomicExch(error_flag, 2);
         return;
     }
+    const int page = slot / p.page, row = slot % p.page;
+    uint16_t* const k_row = p.k_pages + page * p.k_page + (int64_t)row * D;
+    uint16_t* const v_row = p.v_pages + page * p.v_page + (int64_t)row * D;
+    const int64_t head_stride = (int64_t)p.page * D;
+    // items: pairs of eight columns of q, of k, then sixteen columns of v
+    const int q_items = p.n_heads * VEC, k_items = p.n_kv * VEC, items = q_items + 2 * k_items;
+    auto load = [&](int i, uint4& lo, uint4& hi) {
+        if (i < q_items + k_items) {
+            const bool is_q = i < q_items;
+            const int j = is_q ? i : i - q_items, head = j / VEC, d = (j % VEC) * 8;
+            const uint16_t* src = is_q ? p.q + t * p.q_token + head * p.q_head + d : p.k + t * p.k_token + head * p.k_head + d;
+            lo = *reinterpret_cast<const uint4*>(src);
+            hi = *reinterpret_cast<const uint4*>(src + HALF);
+        } else {
+            const int j = i - q_items - k_items, head = j / VEC, d = (j % VEC) * 16;
+            const uint16_t* src = p.v + t * p.v_token + head * p.v_head + d;
+            lo = *reinterpret_cast<const uint4*>(src);
+            hi = *reinterpret_cast<const uint4*>(src + 8);
+        }
+    };
+    uint4 lo = make_uint4(0, 0, 0, 0), hi = lo;
+    if (threadIdx.x < items) load(threadIdx.x, lo, hi);          // on its way while the angles are formed
     if (threadIdx.x < HALF) {
         double turn = (double)p.positions[t] * p.turns[threadIdx.x];
         turn -= rint(turn);
@@ -229,25 +285,24 @@ __global__ void __launch_bounds__(APPEND_THREADS) rope_append_paged_kernel(const
         cs[threadIdx.x] = make_float2(c, sn);
     }
     __syncthreads();
-    const int page = slot / p.page, row = slot % p.page;
-    const int q_items = p.n_heads * VEC, k_items = p.n_kv * VEC, v_items = p.n_kv * 2 * VEC;
-    for (int i = threadIdx.x; i < q_items + k_items + v_items; i += APPEND_THREADS) {
+    for (int i = threadIdx.x; i < items; i += APPEND_THREADS) {
+        uint4 next_lo = lo, next_hi = hi;
+        if (i + APPEND_THREADS < items) load(i + APPEND_THREADS, next_lo, next_hi);
         if (i < q_items + k_items) {
             const bool is_q = i < q_items;
             const int j = is_q ? i : i - q_items, head = j / VEC, d = (j % VEC) * 8;
-            const uint16_t* src = is_q ? p.q + t * p.q_token + head * p.q_head + d : p.k + t * p.k_token + head * p.k_head + d;
-            uint16_t* dst = is_q ? p.q_out + ((int64_t)t * p.n_heads + head) * D + d
-                                 : p.k_pages + page * p.k_page + ((int64_t)head * p.page + row) * D + d;
-            const uint4 lo = *reinterpret_cast<const uint4*>(src), hi = *reinterpret_cast<const uint4*>(src + HALF);
+            uint16_t* dst = is_q ? p.q_out + ((int64_t)t * p.n_heads + head) * D + d : k_row + head * head_stride + d;
             uint4 a, b;
             rotate8<F16>(lo, hi, cs + d, a, b);
             *reinterpret_cast<uint4*>(dst) = a;
             *reinterpret_cast<uint4*>(dst + HALF) = b;
         } else {
-            const int j = i - q_items - k_items, head = j / (2 * VEC), d = (j % (2 * VEC)) * 8;
-            *reinterpret_cast<uint4*>(p.v_pages + page * p.v_page + ((int64_t)head * p.page + row) * D + d) =
-                *reinterpret_cast<const uint4*>(p.v + t * p.v_token + head * p.v_head + d);
+            const int j = i - q_items - k_items, head = j / VEC, d = (j % VEC) * 16;
+            *reinterpret_cast<uint4*>(v_row + head * head_stride + d) = lo;
+            *reinterpret_cast<uint4*>(v_row + head * head_stride + d + 8) = hi;
         }
+        lo = next_lo;
+        hi = next_hi;
     }
 }
 
@@ -279,7 +334,7 @@ int hqm_paged_reserve(int32_t* block_table, int64_t table_stride, int32_t* kv_le
     HQM_CHECK_ARG(tokens >= 0 && tokens <= INT32_MAX, "paged_reserve: %lld tokens", (long long)tokens);
     HQM_CHECK_ARG(cu_seqlens && (sequences == 0 || kv_lens_after) && (tokens == 0 || (positions && slots)), "paged_reserve: null pointer");
     const Tables p{block_table, table_stride, kv_lens, const_cast<int32_t*>(free_pages), free_count, new_lens, cu_seqlens, kv_lens_after,
-                   positions, slots, status, sequences, max_pages, page_size, capacity, tokens};
+                   positions, slots, status, sequences, max_pages, page_size, capacity, tokens, 0};
     return launch_tables(p, true, (cudaStream_t)stream);
 }
 
@@ -291,7 +346,7 @@ int hqm_paged_truncate(const int32_t* block_table, int64_t table_stride, int32_t
                               page_size, capacity))
         return rc;
     const Tables p{const_cast<int32_t*>(block_table), table_stride, kv_lens, free_pages, free_count, keep, nullptr, nullptr, nullptr, nullptr,
-                   status, sequences, max_pages, page_size, capacity, 0};
+                   status, sequences, max_pages, page_size, capacity, 0, 0};
     return launch_tables(p, false, (cudaStream_t)stream);
 }
 

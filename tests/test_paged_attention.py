@@ -278,6 +278,17 @@ def test_many_sequences():
     check(p.paged(), *p.want())
 
 
+@pytest.mark.parametrize("H,n_kv,D,dtype", [(32, 8, 128, torch.bfloat16), (16, 1, 64, torch.float16), (12, 2, 128, torch.float16)])
+def test_single_tokens_beside_chunks(H, n_kv, D, dtype):
+    """Sequences of up to 16 rows per key/value head and longer ones in one call, around that line, empty ones among them."""
+    group = H // n_kv
+    line = 16 // group
+    new = [1] * 20 + [300, 0, line, line + 1, 1, 64, 0, 2, 1] + [1] * 12
+    lens = [n + (37 * i) % 700 for i, n in enumerate(new)]
+    p = Problem(lens, new, H, n_kv, D, 16, dtype)
+    check(p.paged(), *p.want())
+
+
 def test_max_new_is_a_bound_only():
     p = Problem([300, 40, 7], [3, 1, 2], 32, 8, 128, 16, torch.bfloat16)
     want, bound = p.want()

@@ -60,7 +60,7 @@ class Model:
 
 @gpu
 @pytest.mark.parametrize("B,page,pages,most", [(1, 16, 40, 30), (5, 16, 60, 40), (64, 32, 900, 50), (700, 16, 9000, 30), (3, 7, 50, 20),
-                                              (40, 64, 2000, 900)])
+                                              (40, 64, 2000, 900), (3, 16, 2600, 8000)])
 def test_tables_follow_a_plain_model(B, page, pages, most):
     gen = torch.Generator().manual_seed(B)
     order = torch.randperm(pages, generator=gen).tolist()
@@ -128,6 +128,8 @@ def test_no_sequences_and_no_tokens():
     got = paged_reserve(table, none, free, count, none, 16, 3)
     assert got.cu_seqlens.tolist() == [0] and got.slots.tolist() == [-1] * 3 and got.status.item() == 0
     assert paged_truncate(table, none, free, count, none, 16).item() == 0
+    got = paged_reserve(table, none, free, count, none, 16, 5000)
+    assert got.cu_seqlens.tolist() == [0] and got.slots.tolist() == [-1] * 5000 and got.positions.tolist() == [-1] * 5000
     got = paged_reserve(ints([[5, 0]]), ints([3]), free, count, ints([0]), 16, 0)
     assert got.cu_seqlens.tolist() == [0, 0] and got.positions.numel() == 0 and count.item() == 2
 
