@@ -8,6 +8,8 @@
 // warp.  Each warp has its own running maximum, total and sums, so that nothing is exchanged before the end of a unit.  The
 // products go through mma.sync m16n8k16: with 16 rows at the most the matrix unit of tcgen05 would work on 128 rows of which
 // seven eighths are padding, and the bytes, not the products, set the time.
+#include <type_traits>
+
 #include "attn.cuh"
 #include "shared_limit.h"
 #include "tc_common.cuh"
@@ -277,45 +279,67 @@ __global__ void __launch_bounds__(THREADS, 1) attn_few_kernel(const __grid_const
     if (!ok && lane == 0 && error_flag) atomicExch(error_flag, 1);
 }
 
-// CTA (c, y): rows y, y + gridDim.y, ... of the unit whose first piece is CTA c's (of launch `one`, then of `two`), a warp per row.
+// CTA (c, y): rows 8 y .. 8 y + 7 of the unit whose first piece is CTA c's (of launch `one`, then of `two`), a warp per row.  Bound by
+// latency: once the record is there a warp asks for maxima, totals (a lane per piece) and the rows of the first eight
+// pieces at once.
+constexpr int JOIN_ROWS = 8, JOIN_AHEAD = 8;
 template <int D, bool F16>
-__global__ void __launch_bounds__(128) attn_join_kernel(const __grid_constant__ Args one, const __grid_constant__ Args two, int ctas_of_one) {
+__global__ void __launch_bounds__(32 * JOIN_ROWS) attn_join_kernel(const __grid_constant__ Args one, const __grid_constant__ Args two, int ctas_of_one) {
     grid_launch_dependents();
     grid_dependency_wait();
     const Args& a = blockIdx.x < ctas_of_one ? one : two;
     const int c = blockIdx.x < ctas_of_one ? blockIdx.x : blockIdx.x - ctas_of_one, lane = threadIdx.x & 31;
-    const int32_t* rec = a.records + (int64_t)c * RECORD;
-    const int ctas = __ldcg(rec + 4);
-    if (ctas == 0) return;
-    const int q0 = __ldcg(rec), n_rows = __ldcg(rec + 1) * a.group, h = __ldcg(rec + 2), tok0 = __ldcg(rec + 3);
+    const int r = blockIdx.y * JOIN_ROWS + (threadIdx.x >> 5);
+    const int4 rec = __ldcg(reinterpret_cast<const int4*>(a.records + (int64_t)c * RECORD));
+    const int ctas = __ldcg(a.records + (int64_t)c * RECORD + 4);
+    const int q0 = rec.x, n_rows = rec.y * a.group, h = rec.z, tok0 = rec.w;
+    if (ctas == 0 || r >= n_rows) return;
     constexpr int V = D / 32;                                              // columns per lane
-    for (int r = blockIdx.y * 4 + (threadIdx.x >> 5); r < n_rows; r += gridDim.y * 4) {
-        float m = -INFINITY;
-        for (int k = lane; k < ctas; k += 32) m = fmaxf(m, __ldcg(piece_at<D>(a, c + k, k == 0) + a.piece_rows * D + r));
+    typedef typename std::conditional<V == 4, float4, float2>::type Vec;
+    auto piece = [&](int k) { return piece_at<D>(a, c + k, k == 0); };
+    float top = -INFINITY, l = 0.f, x[V] = {};
+    for (int k0 = 0; k0 < ctas; k0 += 32) {
+        const int n = min(32, ctas - k0);
+        float m = -INFINITY, t = 0.f;
+        if (lane < n) {
+            const float* p = piece(k0 + lane);
+            m = __ldcg(p + a.piece_rows * D + r);
+            t = __ldcg(p + a.piece_rows * (D + 1) + r);
+        }
+        Vec v[JOIN_AHEAD];
+        auto ask = [&](int k) {
 #pragma unroll
-        for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-        float l = 0.f, x[V] = {};
-        if (m != -INFINITY) {
-#pragma unroll 4
-            for (int k = 0; k < ctas; ++k) {
-                const float* p = piece_at<D>(a, c + k, k == 0);
-                const float f = ex2(__ldcg(p + a.piece_rows * D + r) - m);
-                l += f * __ldcg(p + a.piece_rows * (D + 1) + r);
-                if constexpr (V == 4) {
-                    const float4 v = __ldcg(reinterpret_cast<const float4*>(p + r * D) + lane);
-                    x[0] += f * v.x; x[1] += f * v.y; x[2] += f * v.z; x[3] += f * v.w;
-                } else {
-                    const float2 v = __ldcg(reinterpret_cast<const float2*>(p + r * D) + lane);
-                    x[0] += f * v.x; x[1] += f * v.y;
+            for (int i = 0; i < JOIN_AHEAD; ++i)
+                if (k + i < n) v[i] = __ldcg(reinterpret_cast<const Vec*>(piece(k0 + k + i) + (int64_t)r * D) + lane);
+        };
+        ask(0);
+        float now = m;
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) now = fmaxf(now, __shfl_xor_sync(0xffffffffu, now, o));
+        now = fmaxf(now, top);
+        const float keep = now == top ? 1.f : ex2(top - now), f = m == -INFINITY ? 0.f : ex2(m - now);
+        top = now;
+        l = l * keep + warp_sum(f * t);
+#pragma unroll
+        for (int e = 0; e < V; ++e) x[e] *= keep;
+        for (int k = 0; k < n; k += JOIN_AHEAD) {
+            if (k > 0) ask(k);
+#pragma unroll
+            for (int i = 0; i < JOIN_AHEAD; ++i) {
+                const float g = __shfl_sync(0xffffffffu, f, (k + i) & 31);
+                if (k + i < n) {
+                    const float* w = reinterpret_cast<const float*>(&v[i]);
+#pragma unroll
+                    for (int e = 0; e < V; ++e) x[e] += g * w[e];
                 }
             }
         }
-        const float inv = m == -INFINITY ? 0.f : 1.f / l;
-        const int64_t row = (int64_t)(q0 + tok0 + r / a.group) * (a.n_kv * a.group) + h * a.group + r % a.group;
-        uint32_t* dst = reinterpret_cast<uint32_t*>(a.out + row * D + V * lane);
-#pragma unroll
-        for (int i = 0; i < V; i += 2) dst[i / 2] = pack2(x[i] * inv, x[i + 1] * inv, F16);
     }
+    const float inv = top == -INFINITY ? 0.f : 1.f / l;
+    const int64_t row = (int64_t)(q0 + tok0 + r / a.group) * (a.n_kv * a.group) + h * a.group + r % a.group;
+    uint32_t* dst = reinterpret_cast<uint32_t*>(a.out + row * D + V * lane);
+#pragma unroll
+    for (int i = 0; i < V; i += 2) dst[i / 2] = pack2(x[i] * inv, x[i + 1] * inv, F16);
 }
 
 template <int D, bool F16>
@@ -340,10 +364,10 @@ int launch_few(const Args& a, const CUtensorMap& km, const CUtensorMap& vm, int 
 
 int launch_join(const Args& a, const Args* more, int ctas, int D, bool f16, cudaStream_t st) {
     const int rows = more && more->piece_rows > a.piece_rows ? more->piece_rows : a.piece_rows;
-    const dim3 grid(more ? 2 * ctas : ctas, (rows + 15) / 16 < 4 ? 4 : (rows + 15) / 16);
+    const dim3 grid(more ? 2 * ctas : ctas, (rows + JOIN_ROWS - 1) / JOIN_ROWS);
     const Args& b = more ? *more : a;
-    if (D == 128) HQM_CUDA(launch_overlapped(f16 ? attn_join_kernel<128, true> : attn_join_kernel<128, false>, grid, 128, 0, st, a, b, ctas));
-    else HQM_CUDA(launch_overlapped(f16 ? attn_join_kernel<64, true> : attn_join_kernel<64, false>, grid, 128, 0, st, a, b, ctas));
+    if (D == 128) HQM_CUDA(launch_overlapped(f16 ? attn_join_kernel<128, true> : attn_join_kernel<128, false>, grid, 32 * JOIN_ROWS, 0, st, a, b, ctas));
+    else HQM_CUDA(launch_overlapped(f16 ? attn_join_kernel<64, true> : attn_join_kernel<64, false>, grid, 32 * JOIN_ROWS, 0, st, a, b, ctas));
     HQM_LAUNCH_CHECK();
     return HQM_OK;
 }
