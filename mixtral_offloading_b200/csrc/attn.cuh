@@ -195,7 +195,8 @@ struct Walk {
     __device__ bool whole() const { return j0 == 0 && j1 == blocks; }
 };
 
-// A piece: sums [rows][D], then maxima [rows] (base 2), then totals [rows].
+// A piece: sums, then maxima [rows] (base 2), then totals [rows].  The sums of attn_few.cu lie as [rows][D]; those of attn_tiles.cu, where
+// neighbouring lanes hold neighbouring rows, as [D / 4][rows][4], so that a warp's store is one stretch.
 template <int D>
 __device__ __forceinline__ float* piece_at(const Args& a, int cta, int tail) {
     return a.pieces + (int64_t)(2 * cta + tail) * a.piece_rows * (D + 2);

@@ -279,21 +279,15 @@ __global__ void __launch_bounds__(THREADS, 1) attn_few_kernel(const __grid_const
     if (!ok && lane == 0 && error_flag) atomicExch(error_flag, 1);
 }
 
-// CTA (c, y): rows 8 y .. 8 y + 7 of the unit whose first piece is CTA c's (of launch `one`, then of `two`), a warp per row.  Bound by
-// latency: once the record is there a warp asks for maxima, totals (a lane per piece) and the rows of the first eight
-// pieces at once.
-constexpr int JOIN_ROWS = 8, JOIN_AHEAD = 8;
+// Bound by latency: maxima, totals and sums of eight pieces are asked for at once.
+constexpr int JOIN_WARPS = 8, JOIN_AHEAD = 8;
+
+// Pieces of attn_few.cu: a warp per row, a lane for D / 32 columns (and for a piece's maximum and total).
 template <int D, bool F16>
-__global__ void __launch_bounds__(32 * JOIN_ROWS) attn_join_kernel(const __grid_constant__ Args one, const __grid_constant__ Args two, int ctas_of_one) {
-    grid_launch_dependents();
-    grid_dependency_wait();
-    const Args& a = blockIdx.x < ctas_of_one ? one : two;
-    const int c = blockIdx.x < ctas_of_one ? blockIdx.x : blockIdx.x - ctas_of_one, lane = threadIdx.x & 31;
-    const int r = blockIdx.y * JOIN_ROWS + (threadIdx.x >> 5);
-    const int4 rec = __ldcg(reinterpret_cast<const int4*>(a.records + (int64_t)c * RECORD));
-    const int ctas = __ldcg(a.records + (int64_t)c * RECORD + 4);
-    const int q0 = rec.x, n_rows = rec.y * a.group, h = rec.z, tok0 = rec.w;
-    if (ctas == 0 || r >= n_rows) return;
+__device__ __forceinline__ void join_few(const Args& a, int c, int ctas, int q0, int n_rows, int h, int tok0) {
+    const int lane = threadIdx.x & 31;
+    const int r = blockIdx.y * JOIN_WARPS + (threadIdx.x >> 5);
+    if (r >= n_rows) return;
     constexpr int V = D / 32;                                              // columns per lane
     typedef typename std::conditional<V == 4, float4, float2>::type Vec;
     auto piece = [&](int k) { return piece_at<D>(a, c + k, k == 0); };
@@ -342,6 +336,62 @@ __global__ void __launch_bounds__(32 * JOIN_ROWS) attn_join_kernel(const __grid_
     for (int i = 0; i < V; i += 2) dst[i / 2] = pack2(x[i] * inv, x[i + 1] * inv, F16);
 }
 
+// Pieces of attn_tiles.cu: CTA y takes rows 32 y .. 32 y + 31, a lane per row and a warp for D / 8 columns; results leave by way of
+// shared memory, a row after another.
+template <int D, bool F16>
+__device__ __forceinline__ void join_tiles(const Args& a, int c, int ctas, int q0, int n_rows, int h, int tok0) {
+    constexpr int COLS = D / JOIN_WARPS, PITCH = D / 2 + 4;                // 32-bit words of a row: 16-byte aligned, on other banks than its neighbours
+    __shared__ uint32_t rows[32 * PITCH];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, r = blockIdx.y * 32 + lane;
+    if (blockIdx.y * 32 >= n_rows) return;
+    const bool valid = r < n_rows;
+    auto piece = [&](int k) { return piece_at<D>(a, c + k, k == 0); };
+    float top = -INFINITY, l = 0.f, x[COLS] = {};
+    for (int k = 0; valid && k < ctas; ++k) {
+        const float* p = piece(k);
+        const float m = __ldcg(p + D * TILE_ROWS + r), t = __ldcg(p + (D + 1) * TILE_ROWS + r);
+        float4 v[COLS / 4];
+#pragma unroll
+        for (int i = 0; i < COLS / 4; ++i) v[i] = __ldcg(reinterpret_cast<const float4*>(p + (warp * COLS + 4 * i) * TILE_ROWS + r * 4));
+        const float now = fmaxf(top, m);
+        const float keep = now == top ? 1.f : ex2(top - now), f = m == -INFINITY ? 0.f : ex2(m - now);
+        top = now;
+        l = l * keep + f * t;
+#pragma unroll
+        for (int i = 0; i < COLS / 4; ++i) {
+            x[4 * i] = x[4 * i] * keep + f * v[i].x;
+            x[4 * i + 1] = x[4 * i + 1] * keep + f * v[i].y;
+            x[4 * i + 2] = x[4 * i + 2] * keep + f * v[i].z;
+            x[4 * i + 3] = x[4 * i + 3] * keep + f * v[i].w;
+        }
+    }
+    const float inv = top == -INFINITY ? 0.f : 1.f / l;
+#pragma unroll
+    for (int i = 0; i < COLS; i += 2) rows[lane * PITCH + (warp * COLS + i) / 2] = pack2(x[i] * inv, x[i + 1] * inv, F16);
+    __syncthreads();
+    for (int i = threadIdx.x; i < 32 * (D / 8); i += 32 * JOIN_WARPS) {
+        const int rr = i / (D / 8), d = i % (D / 8), row = blockIdx.y * 32 + rr;
+        if (row >= n_rows) break;
+        const int64_t at = (int64_t)(q0 + tok0 + row / a.group) * (a.n_kv * a.group) + h * a.group + row % a.group;
+        *reinterpret_cast<uint4*>(a.out + at * D + 8 * d) = *reinterpret_cast<const uint4*>(rows + rr * PITCH + 4 * d);
+    }
+}
+
+// CTA (c, y): of the unit whose first piece is CTA c's, of launch `one`, then of `two`.
+template <int D, bool F16>
+__global__ void __launch_bounds__(32 * JOIN_WARPS) attn_join_kernel(const __grid_constant__ Args one, const __grid_constant__ Args two, int ctas_of_one) {
+    grid_launch_dependents();
+    grid_dependency_wait();
+    const Args& a = blockIdx.x < ctas_of_one ? one : two;
+    const int c = blockIdx.x < ctas_of_one ? blockIdx.x : blockIdx.x - ctas_of_one;
+    const int4 rec = __ldcg(reinterpret_cast<const int4*>(a.records + (int64_t)c * RECORD));
+    const int ctas = __ldcg(a.records + (int64_t)c * RECORD + 4);
+    if (ctas == 0) return;
+    const int n_rows = rec.y * a.group;
+    if (a.piece_rows == TILE_ROWS) join_tiles<D, F16>(a, c, ctas, rec.x, n_rows, rec.z, rec.w);
+    else join_few<D, F16>(a, c, ctas, rec.x, n_rows, rec.z, rec.w);
+}
+
 template <int D, bool F16>
 int few_launch(const Args& a, const CUtensorMap& km, const CUtensorMap& vm, int ctas, cudaStream_t st) {
     constexpr size_t bytes = sizeof(Shared<D>);
@@ -363,11 +413,11 @@ int launch_few(const Args& a, const CUtensorMap& km, const CUtensorMap& vm, int 
 }
 
 int launch_join(const Args& a, const Args* more, int ctas, int D, bool f16, cudaStream_t st) {
-    const int rows = more && more->piece_rows > a.piece_rows ? more->piece_rows : a.piece_rows;
-    const dim3 grid(more ? 2 * ctas : ctas, (rows + JOIN_ROWS - 1) / JOIN_ROWS);
+    const bool tiles = a.piece_rows == TILE_ROWS;                          // (of two launches that is the first)
+    const dim3 grid(more ? 2 * ctas : ctas, tiles ? TILE_ROWS / 32 : FEW_TILE / JOIN_WARPS);
     const Args& b = more ? *more : a;
-    if (D == 128) HQM_CUDA(launch_overlapped(f16 ? attn_join_kernel<128, true> : attn_join_kernel<128, false>, grid, 32 * JOIN_ROWS, 0, st, a, b, ctas));
-    else HQM_CUDA(launch_overlapped(f16 ? attn_join_kernel<64, true> : attn_join_kernel<64, false>, grid, 32 * JOIN_ROWS, 0, st, a, b, ctas));
+    if (D == 128) HQM_CUDA(launch_overlapped(f16 ? attn_join_kernel<128, true> : attn_join_kernel<128, false>, grid, 32 * JOIN_WARPS, 0, st, a, b, ctas));
+    else HQM_CUDA(launch_overlapped(f16 ? attn_join_kernel<64, true> : attn_join_kernel<64, false>, grid, 32 * JOIN_WARPS, 0, st, a, b, ctas));
     HQM_LAUNCH_CHECK();
     return HQM_OK;
 }

@@ -347,7 +347,8 @@ __global__ void __launch_bounds__(THREADS, 1) attn_tiles_kernel(const __grid_con
                     store_32_bytes(a.out + row * D + c + 16, o + 8);
                 } else {
 #pragma unroll
-                    for (int i = 0; i < 32; i += 8) store_32_bytes(piece + pr * D + c + i, o + i);
+                    for (int i = 0; i < 32; i += 4)
+                        *reinterpret_cast<uint4*>(piece + ((c + i) * TILE_ROWS + pr * 4)) = make_uint4(o[i], o[i + 1], o[i + 2], o[i + 3]);
                 }
             }
             fence_before();
