@@ -361,10 +361,11 @@ int hqm_paged_truncate(const int32_t* block_table, int64_t table_stride, int32_t
 /* Rotary embedding (rotate-half) of q and k at every token's position, and the append of k and v at its slot.  Unlike
  * hqm_rope_append_rows, which rounds to bf16 after every operation as Hugging Face does, angles are formed in 64 bits and a
  * result is rounded once.  q (tokens, n_heads, head_dim), k and v (tokens, n_kv_heads, head_dim), strides in elements,
- * multiples of 8, rows 16-byte aligned; q_out (tokens, n_heads, head_dim) contiguous, may be q.  A token whose slot is
- * negative is left out (its row of q_out stays); one beyond the pool is too, and makes hqm_device_error() return 2. */
+ * multiples of 8, rows 16-byte aligned; q_out (tokens, n_heads, head_dim) contiguous, may be q.  k_out (NULL: not wanted): the
+ * rotated k as well, (tokens, n_kv_heads, head_dim) contiguous, may be k; what hqm_prompt_attention wants.  A token whose slot is
+ * negative is left out (its rows of q_out and k_out stay); one beyond the pool is too, and makes hqm_device_error() return 2. */
 typedef struct hqm_paged_append {
-    void* q_out;
+    void *q_out, *k_out;
     const void *q, *k, *v;
     int64_t q_token, q_head, k_token, k_head, v_token, v_head;
     void *k_pages, *v_pages;

@@ -56,7 +56,7 @@ class HqmEpComm(C.Structure):
 class HqmPagedAppend(C.Structure):
     """struct hqm_paged_append."""
     _fields_ = [
-        ("q_out", C.c_void_p), ("q", C.c_void_p), ("k", C.c_void_p), ("v", C.c_void_p),
+        ("q_out", C.c_void_p), ("k_out", C.c_void_p), ("q", C.c_void_p), ("k", C.c_void_p), ("v", C.c_void_p),
         ("q_token", C.c_int64), ("q_head", C.c_int64), ("k_token", C.c_int64), ("k_head", C.c_int64),
         ("v_token", C.c_int64), ("v_head", C.c_int64), ("k_pages", C.c_void_p), ("v_pages", C.c_void_p),
         ("k_page", C.c_int64), ("v_page", C.c_int64), ("positions", C.c_void_p), ("slots", C.c_void_p),

@@ -203,7 +203,7 @@ int launch_tables(Tables p, bool take, cudaStream_t st) {
 
 // ---- append ---------------------------------------------------------------------------------------------------------
 struct Append {
-    uint16_t* q_out;                         // (T, n_heads, D)
+    uint16_t *q_out, *k_out;                 // (T, n_heads, D); (T, n_kv, D) or null
     const uint16_t *q, *k, *v;
     int64_t q_token, q_head, k_token, k_head, v_token, v_head;
     uint16_t *k_pages, *v_pages;             // (pages, n_kv, page, D)
@@ -296,6 +296,11 @@ __global__ void __launch_bounds__(APPEND_THREADS) rope_append_paged_kernel(const
             rotate8<F16>(lo, hi, cs + d, a, b);
             *reinterpret_cast<uint4*>(dst) = a;
             *reinterpret_cast<uint4*>(dst + HALF) = b;
+            if (!is_q && p.k_out) {
+                dst = p.k_out + ((int64_t)t * p.n_kv + head) * D + d;
+                *reinterpret_cast<uint4*>(dst) = a;
+                *reinterpret_cast<uint4*>(dst + HALF) = b;
+            }
         } else {
             const int j = i - q_items - k_items, head = j / VEC, d = (j % VEC) * 16;
             *reinterpret_cast<uint4*>(v_row + head * head_stride + d) = lo;
@@ -366,10 +371,10 @@ int hqm_rope_append_paged(const hqm_paged_append* a, void* stream) {
     if (a->tokens == 0) return HQM_OK;
     HQM_CHECK_ARG(a->q_out && a->q && a->k && a->v && a->k_pages && a->v_pages && a->positions && a->slots, "rope_append_paged: null pointer");
     const int64_t strides = a->q_token | a->q_head | a->k_token | a->k_head | a->v_token | a->v_head | a->k_page | a->v_page;
-    HQM_CHECK_ARG(strides % 8 == 0 && aligned16(a->q_out) && aligned16(a->q) && aligned16(a->k) && aligned16(a->v) && aligned16(a->k_pages) &&
+    HQM_CHECK_ARG(strides % 8 == 0 && aligned16(a->q_out) && aligned16(a->k_out) && aligned16(a->q) && aligned16(a->k) && aligned16(a->v) && aligned16(a->k_pages) &&
                       aligned16(a->v_pages),
                   "rope_append_paged: rows have to start on 16-byte boundaries");
-    Append p{(uint16_t*)a->q_out, (const uint16_t*)a->q, (const uint16_t*)a->k, (const uint16_t*)a->v, a->q_token, a->q_head, a->k_token,
+    Append p{(uint16_t*)a->q_out, (uint16_t*)a->k_out, (const uint16_t*)a->q, (const uint16_t*)a->k, (const uint16_t*)a->v, a->q_token, a->q_head, a->k_token,
              a->k_head, a->v_token, a->v_head, (uint16_t*)a->k_pages, (uint16_t*)a->v_pages, a->k_page, a->v_page, a->positions, a->slots,
              (int)a->tokens, a->n_heads, a->n_kv_heads, a->pages, a->page_size, {}};
     const double step = pow((double)a->rope_theta, -2.0 / a->head_dim);

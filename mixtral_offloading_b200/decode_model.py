@@ -18,6 +18,7 @@ from torch import nn
 
 from .custom_layers import linear_group
 from .decoder import DecoderLayerDecode, add_rmsnorm, greedy_advance, rms_norm_rows, rope_append_rows
+from .paged import paged_attention, paged_reserve, paged_truncate, prompt_attention, rope_append_paged
 from .sampling import sample_token
 
 
@@ -283,3 +284,105 @@ class BatchDecode:
             for fn in self._plan:
                 fn()
         return self._logits
+
+
+class PagedDecode:
+    """Requests of different lengths through the layers of a MixtralDecodeModel (the same weights): prompts, chunks of
+    prompts and single tokens in one step, keys and values in pages that the sequences share (paged.py).
+
+    `sequences` requests at once, a pool of `pages` pages of `page_size` positions per layer, at most `max_len` positions per
+    sequence.  The host keeps the lengths it has asked for, so that it can refuse what does not fit before anything is
+    launched; the tables themselves are made on the device, and nothing in a step waits for it where every layer's
+    MoE block chooses its experts there."""
+
+    def __init__(self, model: MixtralDecodeModel, sequences: int, pages: int, page_size: int = 64, max_len: Optional[int] = None):
+        a0 = model.layers[0].attention
+        dev = model.embed.device
+        self.model, self.page_size, self.pages = model, page_size, pages
+        self.max_len = pages * page_size if max_len is None else max_len
+        shape = (pages, a0.n_kv_heads, page_size, a0.head_dim)
+        self.k_pages = [torch.zeros(shape, dtype=torch.bfloat16, device=dev) for _ in model.layers]
+        self.v_pages = [torch.zeros(shape, dtype=torch.bfloat16, device=dev) for _ in model.layers]
+        self.block_table = torch.zeros((sequences, -(-self.max_len // page_size)), dtype=torch.int32, device=dev)
+        self.kv_lens = torch.zeros((sequences,), dtype=torch.int32, device=dev)
+        self.free_pages = torch.arange(pages - 1, -1, -1, dtype=torch.int32, device=dev)
+        self.free_count = torch.full((1,), pages, dtype=torch.int32, device=dev)
+        self.lens = [0] * sequences                                   # what the device holds once it has got there
+        self.router_logits: List[torch.Tensor] = []
+
+    def _pages(self, lens: Sequence[int]) -> int:
+        return sum(-(-n // self.page_size) for n in lens)
+
+    def _to_device(self, values, dtype) -> torch.Tensor:
+        return torch.tensor(values, dtype=dtype).pin_memory().to(self.model.embed.device, non_blocking=True)
+
+    @torch.inference_mode()
+    def step(self, new_tokens: Sequence[Sequence[int]]) -> torch.Tensor:
+        """new_tokens[b]: the tokens that sequence b is fed, behind what it has (none: it rests).  Returns the logits of the
+        last fed token of every sequence that was fed one, in the order of the sequences (rows, vocab)."""
+        if len(new_tokens) != len(self.lens):
+            raise ValueError(f"tokens of {len(new_tokens)} sequences, not {len(self.lens)}")
+        new = [len(t) for t in new_tokens]
+        after = [a + b for a, b in zip(self.lens, new)]
+        if sum(new) == 0:
+            raise ValueError("a step without tokens")
+        if max(after) > self.max_len or self._pages(after) > self.pages:
+            raise ValueError(f"{sum(new)} new tokens do not fit: {self._pages(after)} of {self.pages} pages, the longest sequence "
+                             f"{max(after)} of {self.max_len}")
+        T, most = sum(new), max(new)
+        ends = [e - 1 for e, n in zip(itertools.accumulate(new), new) if n]
+        ids = self._to_device([int(t) for ts in new_tokens for t in ts], torch.int64)
+        s = paged_reserve(self.block_table, self.kv_lens, self.free_pages, self.free_count, self._to_device(new, torch.int32), self.page_size, T)
+        prompts = all(a == 0 for a, n in zip(self.lens, new) if n)    # nothing cached that they could see
+        self.lens = after
+        h, y, ln_in = self.model.embed[ids], None, self.model.first_ln
+        self.router_logits = []
+        for layer, kp, vp in zip(self.model.layers, self.k_pages, self.v_pages):
+            a = layer.attention
+            q, k, v = linear_group((a.q_proj, a.k_proj, a.v_proj), rms_norm_rows(h, ln_in, a.rms_eps, y))
+            q, k, v = q.view(T, a.n_heads, a.head_dim), k.view(T, a.n_kv_heads, a.head_dim), v.view(T, a.n_kv_heads, a.head_dim)
+            rope_append_paged(q, k, v, kp, vp, s.positions, s.slots, a.rope_theta, out=q, k_out=k if prompts else None)
+            ctx = (prompt_attention(q, k, v, s.cu_seqlens, most) if prompts else
+                   paged_attention(q, kp, vp, self.block_table, s.cu_seqlens, s.kv_lens, most))
+            out = a.o_proj(ctx.view(T, -1))
+            y, logits = layer.moe(rms_norm_rows(out, a.ln_post, a.rms_eps, h).view(1, T, -1))      # out += h
+            h, y, ln_in = out, y.view(T, -1), layer.next_ln
+            self.router_logits.append(logits)
+        rows = self._to_device(ends, torch.int64)
+        x = rms_norm_rows(h[rows], ln_in, self.model.rms_eps, y[rows])
+        return torch.matmul(x, self.model.lm_head.t())
+
+    @torch.inference_mode()
+    def truncate(self, keep: Sequence[int]) -> None:
+        """Sequence b keeps its first keep[b] positions (tokens that were rejected; 0: the request has ended)."""
+        if len(keep) != len(self.lens) or any(not 0 <= k <= n for k, n in zip(keep, self.lens)):
+            raise ValueError(f"sequences of {self.lens} positions cannot keep {list(keep)}")
+        paged_truncate(self.block_table, self.kv_lens, self.free_pages, self.free_count, self._to_device(list(keep), torch.int32), self.page_size)
+        self.lens = [int(k) for k in keep]
+
+    def generate(self, prompts: Sequence[Sequence[int]], new_tokens: int, chunk: int = 512, eos_token_id=None) -> List[List[int]]:
+        """Greedy continuations of the prompts, one per sequence from the first on; prompts longer than `chunk` go in chunks, beside the
+        tokens of those that are generating already.  What the sequences held before is dropped, and so is what they
+        hold in the end."""
+        if not 0 < len(prompts) <= len(self.lens) or any(len(p) == 0 for p in prompts) or chunk < 1 or new_tokens < 1:
+            raise ValueError(f"up to {len(self.lens)} prompts of one token and more")
+        self.truncate([0] * len(self.lens))
+        feed = [list(p) for p in prompts] + [[] for _ in self.lens[len(prompts):]]
+        out: List[List[int]] = [[] for _ in prompts]
+        while any(feed):
+            step = [f[:chunk] for f in feed]
+            feed = [f[chunk:] for f in feed]
+            logits = self.step(step)
+            fed = [b for b, f in enumerate(step) if f]
+            keep = list(self.lens)
+            for b, token in zip(fed, logits.argmax(-1).tolist()):
+                if feed[b]:
+                    continue                                          # in the middle of its prompt
+                out[b].append(token)
+                if len(out[b]) < new_tokens and token != eos_token_id:
+                    feed[b] = [token]
+                else:
+                    keep[b] = 0
+            if keep != self.lens:
+                self.truncate(keep)
+        return out

@@ -484,9 +484,9 @@ bool real(PyObject* obj, float* v) {
     return true;
 }
 
-// rope_append_paged(q, k, v, k_pages, v_pages, positions, slots, theta, out or None)
+// rope_append_paged(q, k, v, k_pages, v_pages, positions, slots, theta, out or None, k_out or None)
 PyObject* rope_append_paged(PyObject*, PyObject* const* args, Py_ssize_t n) {
-    if (n != 9) return PyErr_Format(PyExc_TypeError, "rope_append_paged: nine arguments");
+    if (n != 10) return PyErr_Format(PyExc_TypeError, "rope_append_paged: ten arguments");
     try {
         const at::Tensor* q = queries(args[0]);
         if (q == nullptr) Py_RETURN_NONE;
@@ -502,6 +502,11 @@ PyObject* rope_append_paged(PyObject*, PyObject* const* args, Py_ssize_t n) {
         at::AutoDispatchBelowADInplaceOrView guard;
         at::Tensor out;
         if (!result_like(args[8], *q, &out)) Py_RETURN_NONE;
+        if (args[9] != Py_None) {
+            at::Tensor k_out;
+            if (!result_like(args[9], *k, &k_out)) Py_RETURN_NONE;
+            a.k_out = k_out.data_ptr();
+        }
         a.q_out = out.data_ptr();
         a.q = q->const_data_ptr(), a.k = k->const_data_ptr(), a.v = v->const_data_ptr();
         strides(*q, &a.q_token, &a.q_head);

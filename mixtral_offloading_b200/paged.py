@@ -122,21 +122,22 @@ def _pool(k_pages: torch.Tensor, v_pages: torch.Tensor):
     return pages, n_kv, page_size, k_pages.stride(0) if pages > 1 else one, v_pages.stride(0) if pages > 1 else one
 
 
-def _out(q: torch.Tensor, out: Optional[torch.Tensor]) -> torch.Tensor:
+def _out(q: torch.Tensor, out: Optional[torch.Tensor], name: str = "out") -> torch.Tensor:
     if out is None:
         return torch.empty(q.shape, dtype=q.dtype, device=q.device)
     if out.shape != q.shape or out.dtype != q.dtype or out.device != q.device or not out.is_contiguous():
-        raise ValueError(f"out has to be contiguous, {tuple(q.shape)} {q.dtype} on {q.device}")
+        raise ValueError(f"{name} has to be contiguous, {tuple(q.shape)} {q.dtype} on {q.device}")
     return out
 
 
 def rope_append_paged(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor,
-                      positions: torch.Tensor, slots: torch.Tensor, theta: float, out: Optional[torch.Tensor] = None) -> torch.Tensor:
+                      positions: torch.Tensor, slots: torch.Tensor, theta: float, out: Optional[torch.Tensor] = None,
+                      k_out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """Rotary embedding of q (T, n_heads, head_dim) and k (T, n_kv_heads, head_dim) at `positions` (T,), and append of k and v
     to the pages at `slots` (T,), in one launch (hqm_rope_append_paged).  Returns the rotated q: `out`, which may be q itself, or
-    a new tensor.  Tokens with a negative slot are left out (their rows of `out` stay as they were; of a new tensor they are
-    not initialised).  No two tokens may have the same slot.  Angles in 64 bits, one rounding."""
-    done = _cabi.host().rope_append_paged(q, k, v, k_pages, v_pages, positions, slots, theta, out)
+    a new tensor; k_out, which may be k itself, receives the rotated k as well (prompt_attention wants it).  Tokens with a
+    negative slot are left out (their rows of `out` and `k_out` stay as they were; of a new tensor they are not initialised).  No two tokens may have the same slot.  Angles in 64 bits, one rounding."""
+    done = _cabi.host().rope_append_paged(q, k, v, k_pages, v_pages, positions, slots, theta, out, k_out)
     if done is not None:
         return done
     if q.dim() != 3 or k.dim() != 3 or v.shape != k.shape or q.shape[0] != k.shape[0]:
@@ -150,8 +151,10 @@ def rope_append_paged(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, k_pages
     if positions.shape != (T,) or slots.shape != (T,):
         raise ValueError(f"positions and slots of {T} tokens, not {tuple(positions.shape)} and {tuple(slots.shape)}")
     out = _out(q, out)
+    if k_out is not None:
+        _out(k, k_out, "k_out")
     call = _cabi.HqmPagedAppend(
-        out.data_ptr(), q.data_ptr(), k.data_ptr(), v.data_ptr(), *_strides(q), *_strides(k), *_strides(v), k_pages.data_ptr(),
+        out.data_ptr(), None if k_out is None else k_out.data_ptr(), q.data_ptr(), k.data_ptr(), v.data_ptr(), *_strides(q), *_strides(k), *_strides(v), k_pages.data_ptr(),
         v_pages.data_ptr(), k_page, v_page, positions.data_ptr(), slots.data_ptr(), T, n_heads, n_kv, dim, pages, page_size, code, theta, 0)
     with torch.cuda.device(q.device):
         _cabi.check(_cabi.lib().hqm_rope_append_paged(C.byref(call), _cabi.stream_ptr(q.device)))

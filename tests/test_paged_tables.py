@@ -177,6 +177,12 @@ def test_rope_append(dtype, T, H, n_kv, D, page):
     assert close(kp, want_k, mag) and torch.equal(vp.double(), want_v)
     again = q.contiguous()
     assert torch.equal(rope_append_paged(again, k, v, kp, vp, positions, slots, 1e6, out=again)[~drop], out[~drop])     # in place
+    k_out = torch.full((T, n_kv, D), 6.0, dtype=dtype, device=DEV)
+    assert torch.equal(rope_append_paged(q, k, v, kp, vp, positions, slots, 1e6, k_out=k_out)[~drop], out[~drop])
+    assert torch.equal(k_out[~drop], kp[at // page, :, at % page]) and (k_out[drop] == 6).all()
+    again = k.contiguous()
+    rope_append_paged(q, again, v, kp, vp, positions, slots, 1e6, k_out=again)
+    assert torch.equal(again[~drop], k_out[~drop])
 
 
 @gpu
@@ -253,11 +259,11 @@ def test_the_library_refuses_what_it_cannot_do():
     assert lib.hqm_prompt_attention(None, some, 1 << 40, None) == _cabi.HQM_ERR_ARG
     for change in (dict(tokens=0), dict(sequences=0), dict(max_new=0)):                         # nothing to do
         assert lib.hqm_paged_attention(C.byref(_cabi.HqmAttention(**dict(ok, **change))), None, 0, None) == 0
-    ok = dict(q_out=4096, q=4096, k=4096, v=4096, q_token=512, q_head=128, k_token=256, k_head=128, v_token=256, v_head=128, k_pages=4096,
+    ok = dict(q_out=4096, k_out=0, q=4096, k=4096, v=4096, q_token=512, q_head=128, k_token=256, k_head=128, v_token=256, v_head=128, k_pages=4096,
               v_pages=4096, k_page=4096, v_page=4096, positions=4096, slots=4096, tokens=3, n_heads=4, n_kv_heads=2, head_dim=128, pages=9,
               page_size=16, dtype=0, rope_theta=1e4, reserved=0)
     for change in (dict(head_dim=80), dict(dtype=3), dict(page_size=12), dict(k_page=100), dict(rope_theta=0.0), dict(slots=0), dict(k_head=4),
-                   dict(q=4098), dict(tokens=-1), dict(n_kv_heads=0)):
+                   dict(q=4098), dict(k_out=4100), dict(tokens=-1), dict(n_kv_heads=0)):
         call = _cabi.HqmPagedAppend(**dict(ok, **change))
         assert lib.hqm_rope_append_paged(C.byref(call), None) == _cabi.HQM_ERR_ARG, change
     assert lib.hqm_rope_append_paged(C.byref(_cabi.HqmPagedAppend(**dict(ok, tokens=0))), None) == 0
@@ -300,6 +306,7 @@ def test_the_python_layer_refuses():
         lambda: prompt_attention(q[:, :3], k, k, cu),
         lambda: rope_append_paged(q, k, k, pool, pool, cu, cu, 1e4),
         lambda: rope_append_paged(q, k[:, :1], k[:, :1], pool, pool, ints([0, 1, 2]), ints([0, 1, 2]), 1e4),
+        lambda: rope_append_paged(q, k, k, pool, pool, ints([0, 1, 2]), ints([0, 1, 2]), 1e4, k_out=q),
         lambda: paged_reserve(table, lens, ints([2, 3]), ints([2]), ints([1, 1]), 16, 2),
         lambda: paged_reserve(table, lens, ints([2, 3]), ints([2]), ints([1]), 16, -1),
         lambda: paged_truncate(table, lens, ints([2, 3]), ints([2, 0]), ints([1]), 16),
