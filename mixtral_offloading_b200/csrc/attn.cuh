@@ -37,49 +37,74 @@ struct Args {
 };
 constexpr int RECORD = 8;          // q0, tokens, head, first token, CTAs (0: none), 3 unused
 
-// Sum of floor((a i + b) / m) over i = 0 .. n - 1, for a, b >= 0 (the sum of an arithmetic progression per step of Euclid's algorithm on a, m).
-__host__ __device__ inline int64_t floor_sum(int64_t n, int64_t m, int64_t a, int64_t b) {
+// a / b for a >= 0, b > 0.  (A division of 64 bits is a routine of some 600 cycles.)
+__host__ __device__ inline int64_t quotient(int64_t a, int64_t b) {
+    return (uint64_t)(a | b) >> 32 ? a / b : (int64_t)((uint32_t)a / (uint32_t)b);
+}
+
+// Sum of floor((a i + b) / m) over i = 0 .. n - 1 (the sum of an arithmetic progression per step of Euclid's algorithm on a, m).
+__host__ __device__ inline int64_t floor_sum(int64_t n, uint32_t m, uint32_t a, uint32_t b) {
     int64_t sum = 0;
     while (n > 0) {
         if (a >= m) { sum += (n - 1) * n / 2 * (a / m); a %= m; }
         if (b >= m) { sum += n * (b / m); b %= m; }
-        const int64_t y = a * n + b;
+        const int64_t y = (int64_t)a * n + b;
         if (y < m) break;
-        n = y / m;
-        b = y % m;
-        const int64_t t = m;
+        n = quotient(y, m);
+        b = (uint32_t)(y - n * m);
+        const uint32_t t = m;
         m = a;
         a = t;
     }
     return sum;
 }
 
+// How a kernel cuts the work.
+struct Cut {
+    int per, block_log, extra;     // tokens per tile, log2 of the keys per block, blocks that a unit costs beside its own
+    int per_log;                   // log2 of per, -1 where it is not a power of two
+    __host__ __device__ Cut(int per_, int block_log_, int extra_) : per(per_), block_log(block_log_), extra(extra_), per_log(-1) {
+        if ((per & (per - 1)) == 0)
+            for (per_log = 0; (1 << per_log) < per; ++per_log) {}
+    }
+    __host__ __device__ int tiles(int n) const {           // of n tokens
+        const uint32_t up = (uint32_t)n + per - 1;
+        return (int)(per_log >= 0 ? up >> per_log : up / (uint32_t)per);
+    }
+};
+
 // One sequence's part of the list.
 struct Seq {
     int q0, n;                     // rows of q
     int kv;                        // positions that can be read
     int before;                    // kv - n: what token 0 sees, less one
-    int tiles, per;                // tiles of rows, tokens per tile
-    int block, extra;              // keys per block, blocks that a unit costs beside its own
-    __host__ __device__ int blocks(int tile) const {
-        const int seen = before + min((tile + 1) * per, n);
-        return max(1, (seen + block - 1) / block);
+    int tiles;                     // tiles of rows
+    __host__ __device__ int blocks(const Cut& c, int tile) const {
+        const int seen = before + min((tile + 1) * c.per, n);
+        return max(1, (seen + (1 << c.block_log) - 1) >> c.block_log);
     }
-    // cost of tiles 0 .. count - 1
-    __host__ __device__ int64_t prefix(int count) const {
+    // Cost of tiles 0 .. count - 1.  A tile that sees nothing has one block.  The others of `per` tokens, from tile `empty` on, have
+    // floor((per i + b) / block): where both are powers of two the sum is that of an arithmetic progression in groups of equal terms.
+    __host__ __device__ int64_t prefix(const Cut& c, int count) const {
         const int whole = min(count, tiles - 1);               // tiles of `per` tokens
-        int empty = 0;                                         // of them, the ones that see nothing: one block each
-        if (before < 0) empty = min(whole, (-before) / per);
-        int64_t sum = (int64_t)count * extra + empty + floor_sum(whole - empty, block, per, (int64_t)before + (int64_t)(empty + 1) * per + block - 1);
-        if (count >= tiles && tiles > 0) sum += blocks(tiles - 1);
+        int empty = 0;
+        if (before < 0) empty = min(whole, -before / c.per);
+        int64_t sum = (int64_t)count * c.extra + empty;
+        if (whole > empty) {
+            const int64_t n = whole - empty;
+            const uint32_t b = (uint32_t)((int64_t)before + (int64_t)(empty + 1) * c.per + (1 << c.block_log) - 1);
+            if (c.per_log < 0) sum += floor_sum(n, 1u << c.block_log, c.per, b);
+            else if (c.per_log >= c.block_log) sum += (n * (n - 1) / 2 << (c.per_log - c.block_log)) + n * (b >> c.block_log);
+            else {
+                const int k = c.block_log - c.per_log;         // 2^k tiles of equal blocks
+                auto upto = [k](int64_t x) { const int64_t y = x >> k; return (y * (y - 1) / 2 << k) + (x - (y << k)) * y; };
+                const int64_t first = b >> c.per_log;
+                sum += upto(first + n) - upto(first);
+            }
+        }
+        if (count >= tiles && tiles > 0) sum += blocks(c, tiles - 1);
         return sum;
     }
-    __host__ __device__ int64_t total() const { return prefix(tiles); }
-};
-
-// How a kernel cuts the work.
-struct Cut {
-    int per, block, extra;         // tokens per tile, keys per block, blocks beside a unit's own
 };
 
 __device__ __forceinline__ Seq load_seq(const Args& a, int b, const Cut& c) {
@@ -90,11 +115,8 @@ __device__ __forceinline__ Seq load_seq(const Args& a, int b, const Cut& c) {
     s.kv = s.n;
     if (a.table) s.kv = (int)min((int64_t)max(a.kv_lens[b], 0), (int64_t)a.max_pages << a.page_shift);
     s.before = s.kv - s.n;
-    s.per = c.per;
-    s.block = c.block;
-    s.extra = c.extra;
     const int64_t rows = (int64_t)s.n * a.group;
-    s.tiles = rows > a.rows_above && rows <= a.rows_upto ? (s.n + c.per - 1) / c.per : 0;
+    s.tiles = rows > a.rows_above && rows <= a.rows_upto ? c.tiles(s.n) : 0;
     return s;
 }
 
@@ -104,52 +126,67 @@ struct Run {
     int64_t left;                  // of this one
     int b, h, tile;
     int skip;                      // cost of its first unit that lies in front of the run
+    Seq s;                         // sequence b
 };
 
-// Called by one whole warp; every lane gets the run.
-__device__ inline Run find_run(const Args& a, const Cut& c) {
+// Called by one whole warp; every lane gets the run of CTA `cta` of `ctas`.
+__device__ inline Run find_run(const Args& a, const Cut& c, int cta, int ctas) {
     const int lane = threadIdx.x & 31;
-    int64_t total = 0;
-    for (int b0 = 0; b0 < a.B; b0 += 32) {
-        int64_t w = 0;
-        if (b0 + lane < a.B) w = load_seq(a, b0 + lane, c).total() * a.n_kv;
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1) w += __shfl_xor_sync(0xffffffffu, w, o);
-        total += w;
-    }
-    Run r;
-    r.share = (total + gridDim.x - 1) / gridDim.x;
-    const int64_t lo = r.share * blockIdx.x;
-    r.left = min(max(total - lo, (int64_t)0), r.share);
-    r.b = r.h = r.tile = r.skip = 0;
-    if (r.left == 0) return r;
-    int64_t base = 0;
-    for (int b0 = 0; b0 < a.B; b0 += 32) {
-        int64_t w = 0;
-        if (b0 + lane < a.B) w = load_seq(a, b0 + lane, c).total() * a.n_kv;
-        int64_t sum = w;
+    auto cost = [&](const Seq& s) { return s.prefix(c, s.tiles) * a.n_kv; };
+    // the sequences one round of 32 after another; `sum` of a lane: the cost up to its sequence, within the round
+    Seq mine{};
+    int64_t w = 0, sum = 0;
+    auto round = [&](int b0) {
+        mine = Seq{};
+        if (b0 + lane < a.B) mine = load_seq(a, b0 + lane, c);
+        sum = w = cost(mine);
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
             const int64_t v = __shfl_up_sync(0xffffffffu, sum, o);
             if (lane >= o) sum += v;
         }
+    };
+    int64_t total = 0;
+    for (int b0 = 0; b0 < a.B; b0 += 32) {
+        round(b0);
+        total += __shfl_sync(0xffffffffu, sum, 31);
+    }
+    Run r;
+    r.share = quotient(total + ctas - 1, ctas);
+    const int64_t lo = r.share * cta;
+    r.left = min(max(total - lo, (int64_t)0), r.share);
+    r.b = r.h = r.tile = r.skip = 0;
+    if (r.left == 0) return r;
+    int64_t base = 0;
+    for (int b0 = 0; b0 < a.B; b0 += 32) {
+        if (a.B > 32) round(b0);                               // (else this one was the last)
         const uint32_t past = __ballot_sync(0xffffffffu, base + sum > lo);
         if (past) {
             const int src = __ffs(past) - 1;
             r.b = b0 + src;
             const int64_t off = lo - (base + __shfl_sync(0xffffffffu, sum - w, src));
-            const Seq s = load_seq(a, r.b, c);
-            const int64_t one = s.total();
-            r.h = (int)(off / one);
+            Seq& s = r.s;
+            s.q0 = __shfl_sync(0xffffffffu, mine.q0, src);
+            s.n = __shfl_sync(0xffffffffu, mine.n, src);
+            s.kv = __shfl_sync(0xffffffffu, mine.kv, src);
+            s.before = s.kv - s.n;
+            s.tiles = c.tiles(s.n);
+            const int64_t one = quotient(__shfl_sync(0xffffffffu, w, src), a.n_kv);
+            r.h = (int)quotient(off, one);
             const int64_t in = off - r.h * one;
-            int t0 = 0, t1 = s.tiles - 1;                      // the last tile whose prefix is <= in
-            while (t0 < t1) {
-                const int mid = (t0 + t1 + 1) / 2;
-                if (s.prefix(mid) <= in) t0 = mid;
-                else t1 = mid - 1;
+            // the last tile whose prefix is <= in: of t0 .. t0 + n - 1, 32 places in between at a time
+            int t0 = 0, n = s.tiles;
+            int64_t before = 0;                                // prefix(t0)
+            while (n > 1) {
+                const int step = (n + 31) / 32, t = t0 + lane * step;
+                const int64_t p = lane * step < n ? s.prefix(c, t) : INT64_MAX;
+                const int at = 31 - __clz(__ballot_sync(0xffffffffu, p <= in));
+                before = __shfl_sync(0xffffffffu, p, at);
+                t0 += at * step;
+                n = min(step, n - at * step);
             }
             r.tile = t0;
-            r.skip = (int)(in - s.prefix(t0));
+            r.skip = (int)(in - before);
             return r;
         }
         base += __shfl_sync(0xffffffffu, sum, 31);
@@ -166,9 +203,7 @@ struct Walk {
     int64_t left;
     int b, h, tile, skip;
     int j0, j1, blocks;            // the part: blocks j0 .. j1 - 1 of `blocks`
-    __device__ Walk(const Args& args, const Run& r, const Cut& c) : a(args), cut(c), left(r.left), b(r.b), h(r.h), tile(r.tile), skip(r.skip) {
-        if (left > 0) s = load_seq(a, b, cut);
-    }
+    __device__ Walk(const Args& args, const Run& r, const Cut& c) : a(args), cut(c), s(r.s), left(r.left), b(r.b), h(r.h), tile(r.tile), skip(r.skip) {}
     __device__ bool next() {       // false: done
         while (left > 0) {
             if (tile == s.tiles) {
@@ -179,19 +214,19 @@ struct Walk {
                     while (s.tiles == 0);
                 }
             }
-            blocks = s.blocks(tile++);
-            const int end = (int)min((int64_t)(blocks + s.extra), skip + left);
+            blocks = s.blocks(cut, tile++);
+            const int end = (int)min((int64_t)(blocks + cut.extra), skip + left);
             left -= end - skip;
-            j0 = max(skip - s.extra, 0);
-            j1 = max(end - s.extra, 0);
+            j0 = max(skip - cut.extra, 0);
+            j1 = max(end - cut.extra, 0);
             skip = 0;
             if (j1 > j0) return true;
         }
         return false;
     }
     // the part's tile is tile - 1 from here on
-    __device__ int first_token() const { return (tile - 1) * s.per; }
-    __device__ int tokens() const { return min(s.per, s.n - first_token()); }
+    __device__ int first_token() const { return (tile - 1) * cut.per; }
+    __device__ int tokens() const { return min(cut.per, s.n - first_token()); }
     __device__ bool whole() const { return j0 == 0 && j1 == blocks; }
 };
 
@@ -215,7 +250,7 @@ __device__ __forceinline__ void write_record(const Args& a, const Walk* w, int64
     r[1] = w->tokens();
     r[2] = w->h;
     r[3] = w->first_token();
-    r[4] = 1 + (int)((w->blocks - w->j1 + share - 1) / share);      // this CTA and those that the rest reaches into
+    r[4] = 1 + (int)quotient(w->blocks - w->j1 + share - 1, share);      // this CTA and those that the rest reaches into
 }
 
 __device__ __forceinline__ uint16_t to_bits(float v, bool f16) {
@@ -227,6 +262,7 @@ __device__ __forceinline__ uint32_t pack2(float lo, float hi, bool f16) {      /
     else asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
     return r;
 }
+__device__ __forceinline__ void prefetch_map(const CUtensorMap* m) { asm volatile("prefetch.tensormap [%0];" ::"l"(m) : "memory"); }
 __device__ __forceinline__ float ex2(float x) {
     float r;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
@@ -242,9 +278,9 @@ int launch_few(const Args& a, const CUtensorMap& km, const CUtensorMap& vm, int 
 int launch_tiles(const Args& a, const CUtensorMap& qm, const CUtensorMap& km, const CUtensorMap& vm, int ctas, int D, bool f16, cudaStream_t st);
 
 constexpr int FEW_TILE = 16;       // rows of a unit of attn_few.cu
-constexpr int FEW_KEYS = 64;       // positions of a block there
+constexpr int FEW_KEYS = 64, FEW_KEYS_LOG = 6;         // positions of a block there
 constexpr int TILE_ROWS = 256;     // rows of a unit of attn_tiles.cu
-constexpr int TILE_KEYS = 128;      // positions of a block there
+constexpr int TILE_KEYS = 128, TILE_KEYS_LOG = 7;      // positions of a block there
 constexpr int MIXED_ROWS = 64;     // see attn.cu
 constexpr int MAX_GROUP = 128;     // query heads per key/value head: the rows of a tile
 

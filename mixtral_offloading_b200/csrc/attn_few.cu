@@ -68,18 +68,20 @@ __global__ void __launch_bounds__(THREADS, 1) attn_few_kernel(const __grid_const
     using S = Shared<D>;
     S& sh = *reinterpret_cast<S*>(raw);
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const Cut how{FEW_TILE / a.group, FEW_KEYS, UNIT_EXTRA};
+    const Cut how(FEW_TILE / a.group, FEW_KEYS_LOG, UNIT_EXTRA);
     if (threadIdx.x == 0) {
         for (int i = 0; i < STAGES; ++i) {
             tc::mbar_init(&sh.full[i], 1);
             tc::mbar_init(&sh.empty[i], CONSUMERS / 2);
         }
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+        prefetch_map(&km);
+        prefetch_map(&vm);
     }
     grid_launch_dependents();
     grid_dependency_wait();
     if (warp == 0) {
-        const Run r = find_run(a, how);
+        const Run r = find_run(a, how, blockIdx.x, gridDim.x);
         if (lane == 0) sh.run = r;
     }
     __syncthreads();

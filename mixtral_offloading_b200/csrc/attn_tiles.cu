@@ -5,13 +5,18 @@
 //
 // One CTA per SM works through its run of the list of units (attn.cuh).  A unit is 256 rows, two tiles of 128 (row = token *
 // group + head), over blocks of 128 positions.  Per block and tile two matrix products of 128 x 128 x D are issued, S into
-// tensor memory, and O from p (in tensor memory, over the S that it came from) and V.  A thread of the four warps of a tile
-// owns one row: maximum, total and weights of a row need no other thread.  While one tile's warps form weights the tensor
-// cores work on the other tile's products.
+// tensor memory, and O from p (in tensor memory) and V.  A thread of the four warps of a tile owns one row: maximum, total and
+// weights of a row need no other thread.
 //
-// Warps 0-3: weights of tile 0, 4-7: of tile 1, 8: issues the products, 9: copies (cp.async.bulk.tensor; Q once per unit, K and
-// V of every block through a ring of five buffers, of a paged cache a copy per page), 10: walks the list of units; 11
-// only completes the warpgroup.
+// S does not wait for the weights of the block before: it has columns of its own, and they are free as soon as the tile's warps
+// have S in registers.  With D = 64 both tiles have their own, with D = 128 there is room for one S (128 columns of S, 64 of p
+// per tile, 128 of O per tile: 512), which the tiles take in turns; each needs it for some 900 of the 2600 cycles that a block's
+// weights take.  So the warps that form weights, which set the time, find the next S when they are done with one; where S lay under p
+// they waited for both products of their tile in every block, a third of the time (16001 tokens, 32 on 8 heads of 128: 1.91 ms).
+//
+// Warps 0-3: weights of tile 0, 4-7: of tile 1, 8: issues the products for S, 11: those for O (an issue takes as long as the product, so
+// that one warp for both would leave the tensor cores idle whenever it waits), 9: copies K and V of every block through a ring of
+// five buffers (cp.async.bulk.tensor; of a paged cache a copy per page), 10: walks the list of units and copies their Q.
 //
 // The maximum m that a row's weights refer to is raised only when a block exceeds it by more than 2^8: O, which lies in tensor
 // memory, is rescaled a few times per unit instead of once per block, weights grow to 256 at the most, and l and O mean the same
@@ -34,7 +39,6 @@ constexpr int REGS_WEIGHTS = 216, REGS_OTHERS = 72;
 static_assert(32 * WEIGHT_WARPS * REGS_WEIGHTS + 128 * REGS_OTHERS <= THREADS * 168, "registers of the launch");
 constexpr float SLACK = 8.f;
 constexpr int UNIT_EXTRA = 2;         // what a unit costs beside its blocks, in blocks
-constexpr int BY_POLYNOMIAL = 4;      // of 16 pairs of weights
 
 // A part of a unit (Walk), as the warp that walks the list hands it to the others.
 struct Part {
@@ -42,6 +46,7 @@ struct Part {
     int q_row, head;               // row of q and out of the first token
     int sees, kv;                  // positions that the first token sees, positions of the sequence
     int j0, j1;                    // blocks
+    int end0;                      // blocks j0 .. end0 - 1 hold something that a row of tile 0 sees
     int kv_row, table_row;         // where the sequence begins: packed keys, pages
     int whole;                     // 1: no cut goes through the unit; else 2: its first piece, 0: a later one
 };
@@ -54,9 +59,9 @@ struct Shared {
     static constexpr int TILE = HALVES * PANEL;
     alignas(1024) unsigned char q[2][TILE];
     alignas(1024) unsigned char ring[RING][TILE];                 // K, V, K, V, ...
-    uint64_t full[RING], empty[RING], q_full, q_empty, s_full[2], p_full[2], o_done[2];
+    uint64_t full[RING], empty[RING], q_full[2], q_empty[2], s_full[2], s_read[2], p_full[2], o_done[2];
     uint64_t part_full[PARTS], part_empty[PARTS];
-    Part parts[PARTS];                                            // tokens = 0: the end
+    Part parts[PARTS];
     uint32_t tmem;
 };
 
@@ -118,33 +123,16 @@ __device__ __forceinline__ Pair add2(Pair a, Pair b) {
     asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
     return r;
 }
+// The largest; NaN where one of them is.
 __device__ __forceinline__ float max3(float a, float b, float c) {
     float r;
-    asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+    asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
     return r;
 }
-
-// 2^x without the special-function unit, x up to 2^7: x = n + f with f in [-1/2, 1/2] (the sum with 1.5 2^23 rounds to n), 2^f by
-// the polynomial of least relative error there, n into the exponent.  Off by 7.5e-5 of the value with degree 3 (bf16 rounds
-// by up to 3.9e-3), by 2.6e-6 with degree 4 (fp16: 4.9e-4).  Below 2^-125 the result is 2^-125.
-template <bool F16>
-__device__ __forceinline__ Pair power2(Pair x) {
-    const Pair magic = pair(12582912.f, 12582912.f), unmagic = pair(-12582912.f, -12582912.f), minus = pair(-1.f, -1.f);
-    x = pair(fmaxf(low(x), -125.f), fmaxf(high(x), -125.f));
-    const Pair t = add2(x, magic), n = add2(t, unmagic), f = fma2(n, minus, x);
-    Pair p;
-    if constexpr (F16) {
-        p = fma2(pair(0.00957007613f, 0.00957007613f), f, pair(0.0559178926f, 0.0559178926f));
-        p = fma2(p, f, pair(0.240247458f, 0.240247458f));
-        p = fma2(p, f, pair(0.693121791f, 0.693121791f));
-        p = fma2(p, f, pair(0.999999285f, 0.999999285f));
-    } else {
-        p = fma2(pair(0.0551717728f, 0.0551717728f), f, pair(0.242611378f, 0.242611378f));
-        p = fma2(p, f, pair(0.693260968f, 0.693260968f));
-        p = fma2(p, f, pair(0.999927998f, 0.999927998f));
-    }
-    return pair(__uint_as_float(__float_as_uint(low(p)) + (__float_as_uint(low(t)) << 23)),
-                __uint_as_float(__float_as_uint(high(p)) + (__float_as_uint(high(t)) << 23)));
+__device__ __forceinline__ float max2(float a, float b) {
+    float r;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+    return r;
 }
 
 // V is [position][column]: the product's N runs along a row.  64 columns per 128-byte row; the next 64 a panel further on, the next
@@ -178,9 +166,6 @@ __device__ __forceinline__ void tmem_store16(uint32_t at, const uint32_t* r) {
     asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%16], {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15};" ::HQM_S8(r, 0),
                  HQM_S8(r, 8), "r"(at) : "memory");
 }
-__device__ __forceinline__ void tmem_store8(uint32_t at, const uint32_t* r) {
-    asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%8], {%0,%1,%2,%3,%4,%5,%6,%7};" ::HQM_S8(r, 0), "r"(at) : "memory");
-}
 // The loads of r have arrived.  (The registers go through, so that no use of them moves in front.)
 #define HQM_B8(r, i) "+r"(r[i]), "+r"(r[i + 1]), "+r"(r[i + 2]), "+r"(r[i + 3]), "+r"(r[i + 4]), "+r"(r[i + 5]), "+r"(r[i + 6]), "+r"(r[i + 7])
 __device__ __forceinline__ void loads_done(uint32_t* r) {
@@ -211,18 +196,22 @@ __global__ void __launch_bounds__(THREADS, 1) attn_tiles_kernel(const __grid_con
             tc::mbar_init(&sh.full[i], 1);
             tc::mbar_init(&sh.empty[i], 1);
         }
-        tc::mbar_init(&sh.q_full, 1);
-        tc::mbar_init(&sh.q_empty, 1);
         for (int t = 0; t < 2; ++t) {
+            tc::mbar_init(&sh.q_full[t], 1);
+            tc::mbar_init(&sh.q_empty[t], 1);
             tc::mbar_init(&sh.s_full[t], 1);
+            tc::mbar_init(&sh.s_read[t], WEIGHT_WARPS / 2);
             tc::mbar_init(&sh.p_full[t], WEIGHT_WARPS / 2);
             tc::mbar_init(&sh.o_done[t], 1);
         }
         for (int i = 0; i < PARTS; ++i) {
             tc::mbar_init(&sh.part_full[i], 1);
-            tc::mbar_init(&sh.part_empty[i], WEIGHT_WARPS + 2);
+            tc::mbar_init(&sh.part_empty[i], WEIGHT_WARPS + 3);
         }
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+        prefetch_map(&qm);
+        prefetch_map(&km);
+        prefetch_map(&vm);
     }
     if (warp == WEIGHT_WARPS) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(tc::smem_u32(&sh.tmem)), "r"(512u) : "memory");
@@ -230,6 +219,9 @@ __global__ void __launch_bounds__(THREADS, 1) attn_tiles_kernel(const __grid_con
     }
     grid_launch_dependents();
     grid_dependency_wait();
+    const Cut how(2 * per_tile, TILE_KEYS_LOG, UNIT_EXTRA);
+    Run run;
+    if (warp == WEIGHT_WARPS + 2) run = find_run(a, how, blockIdx.x, gridDim.x);       // while tensor memory is allocated
     fence_before();
     __syncthreads();
     fence_after();
@@ -247,21 +239,24 @@ __global__ void __launch_bounds__(THREADS, 1) attn_tiles_kernel(const __grid_con
         if (lane == 0) tc::mbar_arrive(&sh.part_empty[i]);
         return patience.ok && w.tokens > 0;
     };
-    constexpr uint32_t O_AT = 256;                                 // columns: S 0, 128; O 256, 384
+    // columns of tensor memory
+    constexpr uint32_t S_STEP = D == 64 ? 128 : 0, P_AT = 128 + S_STEP, O_AT = P_AT + 128;
+    constexpr int S_COUNT = D == 64 ? 2 : 1;
     if (warp < WEIGHT_WARPS) {
         // ---- weights: thread = row ----
         asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(REGS_WEIGHTS));
         const int t = warp >> 2, r = threadIdx.x & 127;
         const uint32_t mine = tmem + ((uint32_t)(warp & 3) << 21);
-        const uint32_t s_at = mine + 128 * t, o_at = mine + O_AT + 128 * t;
+        const uint32_t s_at = mine + S_STEP * t, p_at = mine + P_AT + 64 * t, o_at = mine + O_AT + D * t;
         const int tok = t * per_tile + r / a.group;                // within the unit
         uint32_t blocks_done = 0;
         while (next()) {
             if (w.tokens <= t * per_tile) continue;
             const bool valid = r < per_tile * a.group && tok < w.tokens;
             const int limit = valid ? min(w.sees + tok, w.kv) : w.kv;          // positions that the row sees
+            const int end = t == 0 ? w.end0 : w.j1;
             float m = -INFINITY, l = 0.f;
-            for (int j = w.j0; j < w.j1; ++j, ++blocks_done) {
+            for (int j = w.j0; j < end; ++j, ++blocks_done) {
                 patience.wait(&sh.s_full[t], blocks_done & 1);
                 fence_after();
                 uint32_t s[KEYS];
@@ -269,20 +264,28 @@ __global__ void __launch_bounds__(THREADS, 1) attn_tiles_kernel(const __grid_con
                 for (int c = 0; c < KEYS; c += 32) tmem_load32(s + c, s_at + c);
 #pragma unroll
                 for (int c = 0; c < KEYS; c += 32) loads_done(s + c);
+                fence_before();
+                __syncwarp();
+                if (lane == 0) tc::mbar_arrive(&sh.s_read[S_COUNT == 2 ? t : 0]);
                 const int seen = limit - j * KEYS;
                 if (__any_sync(0xffffffffu, seen < KEYS)) {
 #pragma unroll
-                    for (int i = 0; i < KEYS; ++i) s[i] = i < seen ? s[i] : 0xff800000u;
+                    for (int c = 0; c < KEYS; c += 32)
+                        if (__any_sync(0xffffffffu, seen < c + 32)) {
+#pragma unroll
+                            for (int i = c; i < c + 32; ++i) s[i] = i < seen ? s[i] : 0xff800000u;
+                        }
                 }
                 float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
                 for (int i = 0; i < KEYS; i += 8)
 #pragma unroll
                     for (int e = 0; e < 4; ++e) top[e] = max3(top[e], __uint_as_float(s[i + 2 * e]), __uint_as_float(s[i + 2 * e + 1]));
-                const float block_top = fmaxf(max3(top[0], top[1], top[2]), top[3]) * a.scale_log2;
-                const bool raise = block_top > m + SLACK || (m == -INFINITY && block_top > m);
+                const float block_top = max2(max3(top[0], top[1], top[2]), top[3]) * a.scale_log2;
+                const bool raise = valid && !(block_top <= m + SLACK);         // (also of NaN)
                 if (__any_sync(0xffffffffu, raise)) {
-                    const float to = fmaxf(m, block_top);
+                    float to = max2(m, block_top);
+                    if (to == INFINITY) to = NAN;                              // inf - inf, as the definition has it
                     const float f = to == m ? 1.f : ex2(m - to);
                     m = to;
                     l *= f;
@@ -309,11 +312,15 @@ __global__ void __launch_bounds__(THREADS, 1) attn_tiles_kernel(const __grid_con
 #pragma unroll
                     for (int i = 0; i < 16; ++i) {
                         const Pair x = fma2(pair(__uint_as_float(s[c + 2 * i]), __uint_as_float(s[c + 2 * i + 1])), scale2, base2);
-                        const Pair y = (i * BY_POLYNOMIAL) % 16 + BY_POLYNOMIAL >= 16 ? power2<F16>(x) : pair(ex2(low(x)), ex2(high(x)));
+                        const Pair y = pair(ex2(low(x)), ex2(high(x)));
                         sum[i & 1] = add2(sum[i & 1], y);
                         p[i] = pack2(low(y), high(y), F16);
                     }
-                    tmem_store16(s_at + c / 2, p);
+                    if (c == 0 && j > w.j0) {                                  // the product with the weights that lie there is over
+                        patience.wait(&sh.o_done[t], (blocks_done - 1) & 1);
+                        fence_after();
+                    }
+                    tmem_store16(p_at + c / 2, p);
                 }
                 stores_done();
                 fence_before();
@@ -323,8 +330,11 @@ __global__ void __launch_bounds__(THREADS, 1) attn_tiles_kernel(const __grid_con
                 l += low(sum[0]) + high(sum[0]);
             }
             // ---- the part's result ----
-            patience.wait(&sh.o_done[t], (blocks_done - 1) & 1);
-            fence_after();
+            const bool some = w.j0 < end;
+            if (some) {
+                patience.wait(&sh.o_done[t], (blocks_done - 1) & 1);
+                fence_after();
+            }
             const bool whole = w.whole == 1;
             const float inv = m == -INFINITY ? 0.f : 1.f / l;
             const int64_t row = ((int64_t)(w.q_row + tok) * a.n_kv + w.head) * a.group + r % a.group;
@@ -348,7 +358,8 @@ __global__ void __launch_bounds__(THREADS, 1) attn_tiles_kernel(const __grid_con
                 } else {
 #pragma unroll
                     for (int i = 0; i < 32; i += 4)
-                        *reinterpret_cast<uint4*>(piece + ((c + i) * TILE_ROWS + pr * 4)) = make_uint4(o[i], o[i + 1], o[i + 2], o[i + 3]);
+                        *reinterpret_cast<uint4*>(piece + ((c + i) * TILE_ROWS + pr * 4)) =
+                            some ? make_uint4(o[i], o[i + 1], o[i + 2], o[i + 3]) : make_uint4(0, 0, 0, 0);
                 }
             }
             fence_before();
@@ -357,11 +368,10 @@ __global__ void __launch_bounds__(THREADS, 1) attn_tiles_kernel(const __grid_con
         // (A role's code must not come together with one of another number: the compiler counts on the smaller.)
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(REGS_OTHERS));
         if (warp == WEIGHT_WARPS + 1) {
-            // ---- copies ----
+            // ---- copies of K and V ----
             const int rows = a.table ? min(1 << a.page_shift, KEYS) : KEYS;
             const int boxes = KEYS / rows;
-            const uint32_t q_bytes = (uint32_t)(S::HALVES * per_tile * a.group * 128);
-            uint32_t at = 0, units = 0;
+            uint32_t at = 0;
             while (next()) {
                 const int32_t* table = a.table + (int64_t)w.table_row * a.table_stride;
                 for (int j = w.j0; j < w.j1; ++j) {
@@ -387,122 +397,126 @@ __global__ void __launch_bounds__(THREADS, 1) attn_tiles_kernel(const __grid_con
                         }
                         __syncwarp();
                     }
-                    if (j == w.j0) {
-                        // Q behind the first block: what the unit before still multiplies with it does not hold that one up
-                        if (units > 0) patience.wait(&sh.q_empty, (units - 1) & 1);
-                        patience.ok = __all_sync(0xffffffffu, patience.ok);
-                        const int tiles = w.tokens > per_tile ? 2 : 1;
-                        if (patience.ok) {
-                            if (lane == 0) {
-                                expect(&sh.q_full, tiles * q_bytes);
-                                for (int t = 0; t < tiles; ++t)
-#pragma unroll
-                                    for (int h = 0; h < S::HALVES; ++h)
-                                        copy_box(tc::smem_u32(sh.q[t] + h * S::PANEL), &qm, 64 * h, 0, w.head, w.q_row + t * per_tile, &sh.q_full);
-                            }
-                            ++units;
-                        }
-                        __syncwarp();
-                    }
                 }
             }
             // no copy may be on its way when the CTA ends
             Patience last;
             for (uint32_t k = at < RING ? 0 : at - RING; k < at; ++k) last.wait(&sh.full[k % RING], (k / RING) & 1);
-            if (units > 0) last.wait(&sh.q_full, (units - 1) & 1);
         } else if (warp == WEIGHT_WARPS) {
-            // ---- products ----
-            const uint32_t type = F16 ? 0u : (1u << 7) | (1u << 10);
-            const uint32_t idesc_s = (1u << 4) | type | ((KEYS / 8) << 17) | ((128u >> 4) << 24);
-            const uint32_t idesc_o = (1u << 4) | type | (1u << 16) | ((D / 8) << 17) | ((128u >> 4) << 24);
-            uint32_t at = 0, units = 0, p_seen[2] = {0, 0};
-            auto scores = [&](int t, int slot) {                       // S_t = Q_t K^T
-                if (elected()) {
-                    const uint64_t qa = tc::smem_desc_sw128(tc::smem_u32(sh.q[t])), kb = tc::smem_desc_sw128(tc::smem_u32(sh.ring[slot]));
-#pragma unroll
-                    for (int k = 0; k < D / 16; ++k) {
-                        const uint64_t off = ((k >> 2) * S::PANEL + (k & 3) * 32) >> 4;
-                        mma_ss(tmem + 128 * t, qa + off, kb + off, idesc_s, k > 0);
-                    }
-                    tc::umma_commit(&sh.s_full[t]);
-                }
-                __syncwarp();
-            };
+            // ---- S = Q K^T ----
+            const uint32_t idesc = (1u << 4) | (F16 ? 0u : (1u << 7) | (1u << 10)) | ((KEYS / 8) << 17) | ((128u >> 4) << 24);
+            uint32_t at = 0, units[2] = {0, 0}, made[2] = {0, 0};
             while (next()) {
-                const int tiles = w.tokens > per_tile ? 2 : 1;
-                patience.wait(&sh.full[at % RING], (at / RING) & 1);
-                patience.wait(&sh.q_full, units & 1);
-                ++units;
-                fence_after();
-                for (int t = 0; t < tiles; ++t) scores(t, at % RING);
-                if (elected()) {
-                    tc::umma_commit(&sh.empty[at % RING]);
-                    if (w.j1 - w.j0 == 1) tc::umma_commit(&sh.q_empty);
-                }
                 for (int j = w.j0; j < w.j1; ++j, at += 2) {
-                    const int vs = (at + 1) % RING, ks = (at + 2) % RING;
-                    const bool more = j + 1 < w.j1;
-                    patience.wait(&sh.full[vs], ((at + 1) / RING) & 1);
-                    if (more) patience.wait(&sh.full[ks], ((at + 2) / RING) & 1);
-                    const int live = w.kv - j * KEYS;                  // positions of the block that belong to the sequence
+                    const int slot = at % RING;
+                    patience.wait(&sh.full[slot], (at / RING) & 1);
+#pragma unroll
+                    for (int t = 0; t < 2; ++t) {
+                        const int end = t == 0 ? w.end0 : w.tokens > per_tile ? w.j1 : 0;
+                        if (j >= end) continue;
+                        if (j == w.j0) patience.wait(&sh.q_full[t], units[t]++ & 1);
+                        const int buffer = S_COUNT == 2 ? t : 0;
+                        if (made[buffer]++ > 0) patience.wait(&sh.s_read[buffer], made[buffer] & 1);       // (of the one before the last)
+                        fence_after();
+                        if (elected()) {
+                            const uint64_t qa = tc::smem_desc_sw128(tc::smem_u32(sh.q[t])), kb = tc::smem_desc_sw128(tc::smem_u32(sh.ring[slot]));
+#pragma unroll
+                            for (int k = 0; k < D / 16; ++k) {
+                                const uint64_t off = ((k >> 2) * S::PANEL + (k & 3) * 32) >> 4;
+                                mma_ss(tmem + S_STEP * t, qa + off, kb + off, idesc, k > 0);
+                            }
+                            tc::umma_commit(&sh.s_full[t]);
+                            if (j + 1 == end) tc::umma_commit(&sh.q_empty[t]);
+                        }
+                        __syncwarp();
+                    }
+                    if (elected()) tc::umma_commit(&sh.empty[slot]);
+                    __syncwarp();
+                }
+            }
+        } else if (warp == WEIGHT_WARPS + 3) {
+            // ---- O += p V ----
+            const uint32_t idesc = (1u << 4) | (F16 ? 0u : (1u << 7) | (1u << 10)) | (1u << 16) | ((D / 8) << 17) | ((128u >> 4) << 24);
+            uint32_t at = 1, used[2] = {0, 0};
+            while (next()) {
+                for (int j = w.j0; j < w.j1; ++j, at += 2) {
+                    const int slot = at % RING;
+                    patience.wait(&sh.full[slot], (at / RING) & 1);
+                    const int live = w.kv - j * KEYS;                      // positions of the block that belong to the sequence
                     if (live < KEYS) {
                         // behind them lies anything, also NaN, which no weight of zero takes away
                         for (int i = max(live, 0) * 8 + lane; i < KEYS * 8; i += 32)
 #pragma unroll
                             for (int h = 0; h < S::HALVES; ++h)
-                                *reinterpret_cast<uint4*>(sh.ring[vs] + h * S::PANEL + i * 16) = make_uint4(0, 0, 0, 0);
+                                *reinterpret_cast<uint4*>(sh.ring[slot] + h * S::PANEL + i * 16) = make_uint4(0, 0, 0, 0);
                         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                         __syncwarp();
                     }
-                    for (int t = 0; t < tiles; ++t) {
-                        patience.wait(&sh.p_full[t], p_seen[t]++ & 1);
+#pragma unroll
+                    for (int t = 0; t < 2; ++t) {
+                        if (j >= (t == 0 ? w.end0 : w.tokens > per_tile ? w.j1 : 0)) continue;
+                        patience.wait(&sh.p_full[t], used[t]++ & 1);
                         fence_after();
                         if (elected()) {
-                            const uint64_t vb = desc_across(tc::smem_u32(sh.ring[vs]), S::PANEL);
+                            const uint64_t vb = desc_across(tc::smem_u32(sh.ring[slot]), S::PANEL);
 #pragma unroll
                             for (int k = 0; k < KEYS / 16; ++k)
-                                mma_ts(tmem + O_AT + 128 * t, tmem + 128 * t + 8 * k, vb + ((k * 16 * 128) >> 4), idesc_o, j > w.j0 || k > 0);
+                                mma_ts(tmem + O_AT + D * t, tmem + P_AT + 64 * t + 8 * k, vb + ((k * 16 * 128) >> 4), idesc, j > w.j0 || k > 0);
                             tc::umma_commit(&sh.o_done[t]);
                         }
                         __syncwarp();
-                        if (more) scores(t, ks);
                     }
-                    if (elected()) {
-                        tc::umma_commit(&sh.empty[vs]);
-                        if (more) {
-                            tc::umma_commit(&sh.empty[ks]);
-                            if (j + 2 == w.j1) tc::umma_commit(&sh.q_empty);
-                        }
-                    }
+                    if (elected()) tc::umma_commit(&sh.empty[slot]);
                     __syncwarp();
                 }
             }
-        } else if (warp == WEIGHT_WARPS + 2) {
-            // ---- the list ----
-            const Cut how{2 * per_tile, KEYS, UNIT_EXTRA};
-            const Run run = find_run(a, how);
+        } else {
+            // ---- the list, and copies of Q ----
+            const uint32_t q_bytes = (uint32_t)(S::HALVES * per_tile * a.group * 128);
+            uint32_t copies[2] = {0, 0};
             Walk walk(a, run, how);
             bool cut = false, some;
             uint32_t n = 0;
             do {
                 some = walk.next();
                 if (n >= PARTS) patience.wait(&sh.part_empty[n % PARTS], (n / PARTS - 1) & 1);
-                if (some && walk.j0 == 0 && walk.j1 < walk.blocks) {
-                    cut = true;
-                    if (lane == 0) write_record(a, &walk, run.share);
+                Part p{};
+                if (some) {
+                    const int tokens = walk.tokens(), sees = walk.s.before + walk.first_token() + 1;
+                    const int blocks0 = max(1, (sees + min(per_tile, tokens) - 1 + KEYS - 1) / KEYS);
+                    p = Part{tokens, walk.s.q0 + walk.first_token(), walk.h, sees, walk.s.kv, walk.j0, walk.j1, min(blocks0, walk.j1), walk.s.q0, walk.b,
+                             walk.whole() ? 1 : 2 * (walk.j0 == 0)};
                 }
                 if (lane == 0) {
-                    Part p{};
-                    if (some)
-                        p = Part{walk.tokens(), walk.s.q0 + walk.first_token(), walk.h, walk.s.before + walk.first_token() + 1, walk.s.kv, walk.j0,
-                                 walk.j1, walk.s.q0, walk.b, walk.whole() ? 1 : 2 * (walk.j0 == 0)};
                     sh.parts[n % PARTS] = p;
                     tc::mbar_arrive(&sh.part_full[n % PARTS]);
                 }
                 __syncwarp();
+#pragma unroll
+                for (int t = 0; t < 2; ++t) {
+                    if (!some || !(t == 0 ? p.j0 < p.end0 : p.tokens > per_tile)) continue;
+                    if (copies[t] > 0) patience.wait(&sh.q_empty[t], (copies[t] - 1) & 1);
+                    if (!patience.ok) continue;
+                    ++copies[t];
+                    if (lane == 0) {
+                        expect(&sh.q_full[t], q_bytes);
+#pragma unroll
+                        for (int h = 0; h < S::HALVES; ++h)
+                            copy_box(tc::smem_u32(sh.q[t] + h * S::PANEL), &qm, 64 * h, 0, p.head, p.q_row + t * per_tile, &sh.q_full[t]);
+                    }
+                    __syncwarp();
+                }
+                if (some && walk.j0 == 0 && walk.j1 < walk.blocks) {
+                    cut = true;
+                    if (lane == 0) write_record(a, &walk, run.share);
+                }
                 ++n;
             } while (some);
             if (!cut && lane == 0) write_record(a, nullptr, run.share);
+            Patience last;
+#pragma unroll
+            for (int t = 0; t < 2; ++t)
+                if (copies[t] > 0) last.wait(&sh.q_full[t], (copies[t] - 1) & 1);
         }
     }
     if (!patience.ok && lane == 0 && error_flag) atomicExch(error_flag, 1);

@@ -22,6 +22,7 @@ namespace {
 
 constexpr int TABLE_THREADS = 512;
 constexpr int64_t TABLE_ALONE = 4096;
+constexpr int PAGES_AT_ONCE = 4;
 constexpr int MAP_THREADS = 256, MAP_TOKENS = 4 * MAP_THREADS;
 constexpr int MAX_SEQUENCES = 16384;         // three words of shared memory each
 
@@ -37,6 +38,9 @@ struct Tables {
 };
 
 __device__ __forceinline__ int64_t shift_up(int64_t v, int o) { return __shfl_up_sync(0xffffffffu, v, o); }
+
+// Pages of `len` positions.  (In 32 bits, which ceil of 2^31 - 1 fits: a division of 64 bits takes some 600 cycles.)
+__device__ __forceinline__ int pages_of(int len, int page) { return (int)(((uint32_t)len + page - 1) / (uint32_t)page); }
 
 // The last i of 0 .. n - 1 with at[i] <= x (at is not decreasing, at[0] <= x): of equal ones the one whose range holds x.
 __device__ __forceinline__ int range_of(const int32_t* at, int n, int x) {
@@ -71,10 +75,10 @@ __global__ void __launch_bounds__(TABLE_THREADS) tables_kernel(const __grid_cons
         if (b < p.B) {
             const int len = p.lens[b], by = p.change[b];
             const int64_t to = TAKE ? (int64_t)len + by : by;
-            const int64_t most = (int64_t)p.max_pages * p.page;
+            const int64_t row = (int64_t)p.max_pages * p.page, most = row < INT32_MAX ? row : INT32_MAX;
             if (len < 0 || by < 0 || len > most || to > most || (!TAKE && by > len)) s_bad = 1;
             else {
-                const int64_t held = ((int64_t)len + p.page - 1) / p.page, then = (to + p.page - 1) / p.page;
+                const int held = pages_of(len, p.page), then = pages_of((int)to, p.page);
                 v[0] = TAKE ? by : 0;
                 v[1] = TAKE ? then - held : held - then;
             }
@@ -117,19 +121,28 @@ __global__ void __launch_bounds__(TABLE_THREADS) tables_kernel(const __grid_cons
     constexpr int all = TABLE_THREADS;
     __syncthreads();                         // the last read of lengths and count lies in front, their first write behind
     const int top = TAKE ? count - 1 : count + n_pages - 1;
-    for (int i = tid; i < n_pages; i += all) {
-        const int b = range_of(s_pg, p.B, i);
-        const int from = TAKE ? s_len[b] : p.change[b];
-        int32_t* entry = p.table + (int64_t)b * p.stride + (int)(((int64_t)from + p.page - 1) / p.page) + (i - s_pg[b]);
-        if (TAKE) *entry = p.free_pages[top - i];
-        else p.free_pages[top - i] = *entry;
+    for (int i0 = tid; i0 < n_pages; i0 += PAGES_AT_ONCE * all) {
+        int32_t *to[PAGES_AT_ONCE], moved[PAGES_AT_ONCE];
+#pragma unroll
+        for (int k = 0; k < PAGES_AT_ONCE; ++k) {
+            const int i = i0 + k * all;
+            if (i >= n_pages) continue;
+            const int b = range_of(s_pg, p.B, i);
+            int32_t* entry = p.table + (int64_t)b * p.stride + pages_of(TAKE ? s_len[b] : p.change[b], p.page) + (i - s_pg[b]);
+            int32_t* place = p.free_pages + (top - i);
+            to[k] = TAKE ? entry : place;
+            moved[k] = TAKE ? *place : *entry;
+        }
+#pragma unroll
+        for (int k = 0; k < PAGES_AT_ONCE; ++k)
+            if (i0 + k * all < n_pages) *to[k] = moved[k];
     }
     if (TAKE) {
         for (int64_t t = tid; p.maps && t < p.tokens; t += all) {
             int position = -1, slot = -1;
             if (t < n_tokens) {
                 const int b = range_of(s_cu, p.B, (int)t);
-                const int len = s_len[b], held = (int)(((int64_t)len + p.page - 1) / p.page);
+                const int len = s_len[b], held = pages_of(len, p.page);
                 position = len + ((int)t - s_cu[b]);
                 const int i = position / p.page;
                 const int page = i < held ? p.table[(int64_t)b * p.stride + i] : p.free_pages[top - (s_pg[b] + i - held)];
