@@ -91,6 +91,17 @@ struct Kernels {
         return {mixed && c->sequences > 1, true};
     }
 };
+// Whether units are cut.  Where there is a CTA for each and none is long, they are not: the blocks that a CTA then works through one
+// after another cost less than the launch that joins pieces.  What is known here of the lengths are bounds: the table's rows,
+// max_new; the units of a prompt have half as many blocks as the longest on average.  32 on 8 heads of 128, with pieces and
+// whole: one token on 100 positions 8.6 and 6.6 us, on 300 8.7 and 8.3, on 500 9.0 and 10.5; 60 tokens behind 300 14.3 and 12.6, behind 500
+// 15.2 and 16.3; a prompt of 250 tokens 14.9 and 11.7, of 500 17.4 and 15.0, of 700 20.8 and 18.2.
+bool cuts(const hqm_attention* c, bool paged, int ctas, int per, int block, int most_blocks) {
+    const int64_t most = c->max_new < c->tokens ? c->max_new : c->tokens;
+    const int64_t positions = paged ? (int64_t)c->max_pages * c->page_size : most, blocks = (positions + block - 1) / block;
+    const int64_t units = (c->tokens / per + c->sequences) * c->n_kv_heads;
+    return blocks > 1 && (units > ctas || (paged ? blocks : (blocks + 1) / 2) > most_blocks);
+}
 size_t launch_bytes(int ctas, int rows, int D) { return record_bytes(ctas) + (piece_bytes(ctas, rows, D) + 255) / 256 * 256; }
 
 int run(const hqm_attention* c, bool paged, const char* what, void* scratch, size_t scratch_bytes, void* stream) {
@@ -133,6 +144,8 @@ int run(const hqm_attention* c, bool paged, const char* what, void* scratch, siz
         at += launch_bytes(ctas, rows, D);
     };
     const Kernels k = Kernels::of(c, paged);
+    few.cuts = cuts(c, paged, ctas, FEW_TILE / a.group > 0 ? FEW_TILE / a.group : 1, FEW_KEYS, FEW_WHOLE);
+    tiles.cuts = cuts(c, paged, ctas, TILE_ROWS / 2 / a.group * 2, TILE_KEYS, TILES_WHOLE);
     few.rows_above = tiles.rows_above = 0;
     few.rows_upto = tiles.rows_upto = INT32_MAX;
     if (k.few && k.tiles) few.rows_upto = tiles.rows_above = FEW_TILE;
@@ -152,7 +165,7 @@ int run(const hqm_attention* c, bool paged, const char* what, void* scratch, siz
         return HQM_ERR_CUDA;
     };
     const cudaStream_t st = (cudaStream_t)stream;
-    CUtensorMap qm, km, vm;
+    CUtensorMap qm, km, vm, kf, vf;
     if (k.tiles) {
         place(tiles, TILE_ROWS);
         // row = token * group + head: a box of all heads of a group and as many tokens as a tile holds
@@ -160,13 +173,16 @@ int run(const hqm_attention* c, bool paged, const char* what, void* scratch, siz
         const int64_t strides[3] = {c->q_head, c->q_head * a.group, c->q_token};
         const cuuint32_t box[4] = {64, (cuuint32_t)a.group, 1, 128u / a.group};
         if (!maps(&km, &vm, TILE_KEYS, false) || !encode(&qm, c->q, 4, dims, strides, box, f16)) return no_maps();
-        if (int rc = launch_tiles(tiles, qm, km, vm, ctas, D, f16, st)) return rc;
     }
     if (k.few) {
         place(few, FEW_TILE);
-        if (!maps(&km, &vm, FEW_KEYS, true)) return no_maps();
-        if (int rc = launch_few(few, km, vm, ctas, D, f16, st)) return rc;
+        if (!maps(&kf, &vf, FEW_KEYS, true)) return no_maps();
     }
+    const int rc = k.few && k.tiles ? launch_mixed(tiles, few, qm, km, vm, kf, vf, ctas, D, f16, st)
+                   : k.few          ? launch_few(few, kf, vf, ctas, D, f16, st)
+                                    : launch_tiles(tiles, qm, km, vm, ctas, D, f16, st);
+    if (rc) return rc;
+    if (!(k.tiles && tiles.cuts) && !(k.few && few.cuts)) return HQM_OK;
     return launch_join(k.tiles ? tiles : few, k.tiles && k.few ? &few : nullptr, ctas, D, f16, st);
 }
 

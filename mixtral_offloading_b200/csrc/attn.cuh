@@ -34,6 +34,7 @@ struct Args {
     int32_t* records;              // of CTA c: the unit that starts in c and is cut behind it (RECORD words)
     int piece_rows;                // rows of a piece
     int rows_above, rows_upto;     // the launch is about sequences with that many rows per key/value head
+    int cuts;                      // 0: a CTA takes the units that begin in its run as a whole, and there is nothing to join
 };
 constexpr int RECORD = 8;          // q0, tokens, head, first token, CTAs (0: none), 3 unused
 
@@ -129,6 +130,18 @@ struct Run {
     Seq s;                         // sequence b
 };
 
+// Cost of the whole list.  Called by one whole warp.
+__device__ inline int64_t total_cost(const Args& a, const Cut& c) {
+    int64_t total = 0;
+    for (int b = threadIdx.x & 31; b < a.B; b += 32) {
+        const Seq s = load_seq(a, b, c);
+        total += s.prefix(c, s.tiles);
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
+    return total * a.n_kv;
+}
+
 // Called by one whole warp; every lane gets the run of CTA `cta` of `ctas`.
 __device__ inline Run find_run(const Args& a, const Cut& c, int cta, int ctas) {
     const int lane = threadIdx.x & 31;
@@ -215,6 +228,15 @@ struct Walk {
                 }
             }
             blocks = s.blocks(cut, tile++);
+            if (!a.cuts) {
+                const bool begins = skip == 0;
+                left -= blocks + cut.extra - skip;
+                skip = 0;
+                j0 = 0;
+                j1 = blocks;
+                if (begins) return true;
+                continue;
+            }
             const int end = (int)min((int64_t)(blocks + cut.extra), skip + left);
             left -= end - skip;
             j0 = max(skip - cut.extra, 0);
@@ -240,8 +262,8 @@ inline size_t piece_bytes(int ctas, int rows, int D) { return (size_t)2 * ctas *
 inline size_t record_bytes(int ctas) { return ((size_t)ctas * RECORD * sizeof(int32_t) + 255) / 256 * 256; }
 
 // CTA c's record: about the unit that its run ends in the middle of and that began in it, if there is one.
-__device__ __forceinline__ void write_record(const Args& a, const Walk* w, int64_t share) {
-    int32_t* r = a.records + (int64_t)blockIdx.x * RECORD;
+__device__ __forceinline__ void write_record(const Args& a, const Walk* w, int64_t share, int cta) {
+    int32_t* r = a.records + (int64_t)cta * RECORD;
     if (!w) {
         r[4] = 0;
         return;
@@ -276,12 +298,16 @@ int launch_few(const Args& a, const CUtensorMap& km, const CUtensorMap& vm, int 
 
 // attn_tiles.cu: any number.
 int launch_tiles(const Args& a, const CUtensorMap& qm, const CUtensorMap& km, const CUtensorMap& vm, int ctas, int D, bool f16, cudaStream_t st);
+// Both at once, f about the sequences of few rows.
+int launch_mixed(const Args& a, const Args& f, const CUtensorMap& qm, const CUtensorMap& km, const CUtensorMap& vm, const CUtensorMap& kf,
+                 const CUtensorMap& vf, int ctas, int D, bool f16, cudaStream_t st);
 
 constexpr int FEW_TILE = 16;       // rows of a unit of attn_few.cu
 constexpr int FEW_KEYS = 64, FEW_KEYS_LOG = 6;         // positions of a block there
 constexpr int TILE_ROWS = 256;     // rows of a unit of attn_tiles.cu
 constexpr int TILE_KEYS = 128, TILE_KEYS_LOG = 7;      // positions of a block there
 constexpr int MIXED_ROWS = 64;     // see attn.cu
+constexpr int FEW_WHOLE = 5, TILES_WHOLE = 4;              // blocks, see attn.cu
 constexpr int MAX_GROUP = 128;     // query heads per key/value head: the rows of a tile
 
 }  // namespace attn

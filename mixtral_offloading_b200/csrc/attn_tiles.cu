@@ -23,9 +23,8 @@
 // whatever m is.
 #include <type_traits>
 
-#include "attn.cuh"
+#include "attn_few.cuh"
 #include "shared_limit.h"
-#include "tc_common.cuh"
 
 namespace hqm {
 namespace attn {
@@ -182,13 +181,13 @@ __device__ __forceinline__ bool elected() {
     return one != 0;
 }
 
-template <int D, bool F16>
-__global__ void __launch_bounds__(THREADS, 1) attn_tiles_kernel(const __grid_constant__ CUtensorMap qm, const __grid_constant__ CUtensorMap km,
-                                                                const __grid_constant__ CUtensorMap vm, const __grid_constant__ Args a,
-                                                                int* error_flag) {
-    extern __shared__ __align__(1024) unsigned char raw[];
+__device__ __forceinline__ Cut cut(const Args& a) { return Cut(128 / a.group * 2, TILE_KEYS_LOG, UNIT_EXTRA); }
+
+// What CTA `cta` of `ctas` does.  FIRST: nothing has waited for the grid in front yet.
+template <int D, bool F16, bool FIRST>
+__device__ __forceinline__ void tiles_cta(Shared<D>& sh, const CUtensorMap& qm, const CUtensorMap& km, const CUtensorMap& vm, const Args& a, int cta,
+                                          int ctas, int* error_flag) {
     using S = Shared<D>;
-    S& sh = *reinterpret_cast<S*>(raw);
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int per_tile = 128 / a.group;                            // tokens
     if (threadIdx.x == 0) {
@@ -217,11 +216,13 @@ __global__ void __launch_bounds__(THREADS, 1) attn_tiles_kernel(const __grid_con
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(tc::smem_u32(&sh.tmem)), "r"(512u) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     }
-    grid_launch_dependents();
-    grid_dependency_wait();
-    const Cut how(2 * per_tile, TILE_KEYS_LOG, UNIT_EXTRA);
+    if constexpr (FIRST) {
+        grid_launch_dependents();
+        grid_dependency_wait();
+    }
+    const Cut how = cut(a);
     Run run;
-    if (warp == WEIGHT_WARPS + 2) run = find_run(a, how, blockIdx.x, gridDim.x);       // while tensor memory is allocated
+    if (warp == WEIGHT_WARPS + 2) run = find_run(a, how, cta, ctas);       // while tensor memory is allocated
     fence_before();
     __syncthreads();
     fence_after();
@@ -339,7 +340,7 @@ __global__ void __launch_bounds__(THREADS, 1) attn_tiles_kernel(const __grid_con
             const float inv = m == -INFINITY ? 0.f : 1.f / l;
             const int64_t row = ((int64_t)(w.q_row + tok) * a.n_kv + w.head) * a.group + r % a.group;
             const int pr = t * per_tile * a.group + r;
-            float* piece = piece_at<D>(a, blockIdx.x, w.whole >> 1);
+            float* piece = piece_at<D>(a, cta, w.whole >> 1);
             if (valid && !whole) {
                 piece[a.piece_rows * D + pr] = m;
                 piece[a.piece_rows * (D + 1) + pr] = l;
@@ -475,7 +476,7 @@ __global__ void __launch_bounds__(THREADS, 1) attn_tiles_kernel(const __grid_con
             const uint32_t q_bytes = (uint32_t)(S::HALVES * per_tile * a.group * 128);
             uint32_t copies[2] = {0, 0};
             Walk walk(a, run, how);
-            bool cut = false, some;
+            bool split = false, some;
             uint32_t n = 0;
             do {
                 some = walk.next();
@@ -507,12 +508,12 @@ __global__ void __launch_bounds__(THREADS, 1) attn_tiles_kernel(const __grid_con
                     __syncwarp();
                 }
                 if (some && walk.j0 == 0 && walk.j1 < walk.blocks) {
-                    cut = true;
-                    if (lane == 0) write_record(a, &walk, run.share);
+                    split = true;
+                    if (lane == 0) write_record(a, &walk, run.share, cta);
                 }
                 ++n;
             } while (some);
-            if (!cut && lane == 0) write_record(a, nullptr, run.share);
+            if (!split && lane == 0) write_record(a, nullptr, run.share, cta);
             Patience last;
 #pragma unroll
             for (int t = 0; t < 2; ++t)
@@ -529,16 +530,82 @@ __global__ void __launch_bounds__(THREADS, 1) attn_tiles_kernel(const __grid_con
 }
 
 template <int D, bool F16>
-int tiles_launch(const Args& a, const CUtensorMap& qm, const CUtensorMap& km, const CUtensorMap& vm, int ctas, cudaStream_t st) {
-    constexpr size_t bytes = sizeof(Shared<D>);
-    static SharedLimits limits;
-    if (!allow_shared(attn_tiles_kernel<D, F16>, limits, bytes)) {
+__global__ void __launch_bounds__(THREADS, 1) attn_tiles_kernel(const __grid_constant__ CUtensorMap qm, const __grid_constant__ CUtensorMap km,
+                                                                const __grid_constant__ CUtensorMap vm, const __grid_constant__ Args a,
+                                                                int* error_flag) {
+    extern __shared__ __align__(1024) unsigned char raw[];
+    tiles_cta<D, F16, true>(*reinterpret_cast<Shared<D>*>(raw), qm, km, vm, a, blockIdx.x, gridDim.x, error_flag);
+}
+
+// Single tokens beside chunks: the first CTAs work on the sequences of many rows (a: bound by weights and products), the others on
+// those of few (f: bound by the bytes), at the same time.  How many: so that both take as long, from the lengths; a block of 128
+// positions and 256 rows is taken for MIXED_COST blocks of 64 positions and few rows.  Two chunks of up to 512 tokens among 30 single
+// ones, 32 on 8 heads of 128: 96 us in two launches one after the other; 81, 78, 82 and 96 us with a cost of 2, 3, 4 and 6.
+constexpr int MIXED_COST = 3;
+
+template <int D, bool F16>
+__global__ void __launch_bounds__(THREADS, 1)
+    attn_mixed_kernel(const __grid_constant__ CUtensorMap qm, const __grid_constant__ CUtensorMap km, const __grid_constant__ CUtensorMap vm,
+                      const __grid_constant__ CUtensorMap kf, const __grid_constant__ CUtensorMap vf, const __grid_constant__ Args a,
+                      const __grid_constant__ Args f, int* error_flag) {
+    extern __shared__ __align__(1024) unsigned char raw[];
+    __shared__ int64_t cost[2];
+    const int warp = threadIdx.x >> 5, cta = blockIdx.x, ctas = gridDim.x;
+    grid_launch_dependents();
+    grid_dependency_wait();
+    if (warp < 2) {
+        const int64_t total = warp == 0 ? total_cost(a, cut(a)) * MIXED_COST : total_cost(f, few::cut(f));
+        if ((threadIdx.x & 31) == 0) cost[warp] = total;
+    }
+    __syncthreads();
+    const int64_t all = cost[0] + cost[1];
+    int first = ctas;                                              // CTAs of the many rows
+    if (cost[0] == 0) first = 0;
+    else if (cost[1] > 0) first = min(max((int)((float)ctas * (float)cost[0] / (float)all + 0.5f), 1), ctas - 1);
+    if (cta < first) {
+        if (threadIdx.x == 0) f.records[(int64_t)(ctas - first + cta) * RECORD + 4] = 0;
+        tiles_cta<D, F16, false>(*reinterpret_cast<Shared<D>*>(raw), qm, km, vm, a, cta, first, error_flag);
+    } else {
+        if (threadIdx.x == 0) a.records[(int64_t)cta * RECORD + 4] = 0;
+        auto& sh = *reinterpret_cast<few::Shared<D>*>(raw);
+        few::begin<D>(sh, kf, vf);
+        if (warp == 0) {
+            const Run r = find_run(f, few::cut(f), cta - first, ctas - first);
+            if (threadIdx.x == 0) sh.run = r;
+        }
+        __syncthreads();
+        if (warp < few::CONSUMERS) {
+            asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(REGS_WEIGHTS));
+            few::products<D, F16>(sh, f, cta - first, error_flag);
+        } else {
+            asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(REGS_OTHERS));
+            if (warp == few::CONSUMERS) few::copies<D>(sh, kf, vf, f, error_flag);
+        }
+    }
+}
+static_assert(few::CONSUMERS == WEIGHT_WARPS && few::THREADS <= THREADS, "attn_mixed_kernel: the warpgroups of both kinds");
+
+template <typename K, typename... A>
+int start(K kernel, SharedLimits& limits, size_t bytes, int ctas, cudaStream_t st, const A&... args) {
+    if (!allow_shared(kernel, limits, bytes)) {
         set_error("attention: a CTA cannot have %zu bytes of shared memory", bytes);
         return HQM_ERR_CUDA;
     }
-    HQM_CUDA(launch_overlapped(attn_tiles_kernel<D, F16>, ctas, THREADS, bytes, st, qm, km, vm, a, tc_error_ptr()));
+    HQM_CUDA(launch_overlapped(kernel, ctas, THREADS, bytes, st, args..., tc_error_ptr()));
     HQM_LAUNCH_CHECK();
     return HQM_OK;
+}
+template <int D, bool F16>
+int tiles_launch(const Args& a, const CUtensorMap& qm, const CUtensorMap& km, const CUtensorMap& vm, int ctas, cudaStream_t st) {
+    static SharedLimits limits;
+    return start(attn_tiles_kernel<D, F16>, limits, sizeof(Shared<D>), ctas, st, qm, km, vm, a);
+}
+template <int D, bool F16>
+int mixed_launch(const Args& a, const Args& f, const CUtensorMap& qm, const CUtensorMap& km, const CUtensorMap& vm, const CUtensorMap& kf,
+                 const CUtensorMap& vf, int ctas, cudaStream_t st) {
+    static SharedLimits limits;
+    constexpr size_t bytes = sizeof(Shared<D>) > sizeof(few::Shared<D>) ? sizeof(Shared<D>) : sizeof(few::Shared<D>);
+    return start(attn_mixed_kernel<D, F16>, limits, bytes, ctas, st, qm, km, vm, kf, vf, a, f);
 }
 
 }  // namespace
@@ -546,6 +613,12 @@ int tiles_launch(const Args& a, const CUtensorMap& qm, const CUtensorMap& km, co
 int launch_tiles(const Args& a, const CUtensorMap& qm, const CUtensorMap& km, const CUtensorMap& vm, int ctas, int D, bool f16, cudaStream_t st) {
     if (D == 128) return f16 ? tiles_launch<128, true>(a, qm, km, vm, ctas, st) : tiles_launch<128, false>(a, qm, km, vm, ctas, st);
     return f16 ? tiles_launch<64, true>(a, qm, km, vm, ctas, st) : tiles_launch<64, false>(a, qm, km, vm, ctas, st);
+}
+
+int launch_mixed(const Args& a, const Args& f, const CUtensorMap& qm, const CUtensorMap& km, const CUtensorMap& vm, const CUtensorMap& kf,
+                 const CUtensorMap& vf, int ctas, int D, bool f16, cudaStream_t st) {
+    if (D == 128) return f16 ? mixed_launch<128, true>(a, f, qm, km, vm, kf, vf, ctas, st) : mixed_launch<128, false>(a, f, qm, km, vm, kf, vf, ctas, st);
+    return f16 ? mixed_launch<64, true>(a, f, qm, km, vm, kf, vf, ctas, st) : mixed_launch<64, false>(a, f, qm, km, vm, kf, vf, ctas, st);
 }
 
 }  // namespace attn
