@@ -83,28 +83,33 @@ __device__ __forceinline__ void copies(Shared<D>& sh, const CUtensorMap& km, con
     const int lane = threadIdx.x & 31;
     Walk w(a, sh.run, cut(a));
     bool ok = true;
-    const int rows = a.table ? min(1 << a.page_shift, FEW_KEYS) : FEW_KEYS, boxes = FEW_KEYS / rows;       // of a box, per block
+    const int rows_log = a.table ? min(a.page_shift, FEW_KEYS_LOG) : FEW_KEYS_LOG, rows = 1 << rows_log;         // of a box
+    const int boxes_log = FEW_KEYS_LOG - rows_log, boxes = 1 << boxes_log;                                     // per block
     {
         uint32_t at = 0;
         while (w.next() && ok) {
             const int32_t* table = a.table + (int64_t)w.b * a.table_stride;
-            // of block j; read one block ahead of the copies
-            auto place = [&](int j, int& row, int& page) {
-                const int key = j * FEW_KEYS + lane * rows;
-                row = w.s.q0 + key;
-                page = 0;
-                if (!a.table || lane >= boxes || key >= w.s.kv) return;
-                page = min((uint32_t)table[key >> a.page_shift], (uint32_t)a.n_pages);           // outside the pool: zeros
-                row = key & ((1 << a.page_shift) - 1);
+            // Entries of the table, 32 at once and a round ahead of the copies (one that waits for its entry takes some 800 cycles; 130001
+            // positions: 98 us when an entry was read one block ahead, 93 so): lane i has that of box i % boxes of block from + i / boxes.
+            auto entries = [&](int from) {
+                const int j = from + (lane >> boxes_log), key = j * FEW_KEYS + (lane & (boxes - 1)) * rows;
+                if (!a.table || j >= w.j1 || key >= w.s.kv) return 0;
+                return (int)min((uint32_t)table[key >> a.page_shift], (uint32_t)a.n_pages);      // outside the pool: zeros
             };
-            int row, page, next_row = 0, next_page = 0;
-            place(w.j0, row, page);
-            for (int j = w.j0; j < w.j1 && ok; ++j, ++at, row = next_row, page = next_page) {
-                if (j + 1 < w.j1) place(j + 1, next_row, next_page);
+            const int round = 32 >> boxes_log;
+            int now = 0, ahead = entries(w.j0);
+            for (int j = w.j0; j < w.j1 && ok; ++j, ++at) {
+                const int in = (j - w.j0) & (round - 1);
+                if (in == 0) {
+                    now = ahead;
+                    ahead = entries(j + round);
+                }
+                const int page = __shfl_sync(0xffffffffu, now, (in * boxes + lane) & 31);
+                const int key = j * FEW_KEYS + lane * rows, row = a.table ? key & ((1 << a.page_shift) - 1) : w.s.q0 + key;
                 const int stage = at % STAGES;
                 if (at >= STAGES) ok = __all_sync(0xffffffffu, tc::mbar_wait(&sh.empty[stage], (at / STAGES - 1) & 1));
                 if (!ok) break;
-                const int live = min(boxes, (max(w.s.kv - j * FEW_KEYS, 0) + rows - 1) / rows);  // boxes that hold positions of the sequence
+                const int live = min(boxes, (max(w.s.kv - j * FEW_KEYS, 0) + rows - 1) >> rows_log);  // boxes that hold positions of the sequence
                 const uint32_t bar = tc::smem_u32(&sh.full[stage]);
                 if (lane == 0) expect(bar, (uint32_t)live * rows * 128 * S::HALVES * 2);
                 __syncwarp();
@@ -135,7 +140,8 @@ __device__ __forceinline__ void products(Shared<D>& sh, const Args& a, int cta, 
     auto key_at = [&](int key) { return (uint32_t)(((key & ~(rows - 1)) * (D / 64) + (key & (rows - 1))) * 128); };
     const int across = rows * 128;
     const int krow = strip + (lane & 7) + ((lane >> 4) << 3), kch = (lane >> 3) & 1, vrow = strip + (lane & 15), vch = lane >> 4;
-    const uint32_t k_off = key_at(krow), v_off = key_at(vrow);
+    // (16-byte columns of a row lie at their number xor the row's: those of step k at the first step's address xor 32 k)
+    const uint32_t k_off = key_at(krow) + ((kch ^ (krow & 7)) << 4), v_off = key_at(vrow) + ((vch ^ (vrow & 7)) << 4);
     uint32_t at = 0;
     bool split = false;
     while (w.next()) {
@@ -145,7 +151,7 @@ __device__ __forceinline__ void products(Shared<D>& sh, const Args& a, int cta, 
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
             const int r = r0 + 8 * i, tok = tok0 + r / a.group;
-            limit[i] = r < n_rows ? w.s.before + tok + 1 : 0;
+            limit[i] = r < n_rows ? w.s.before + tok + 1 : w.s.kv;              // (a row of padding is nobody's)
             const uint16_t* src = a.q + (int64_t)(w.s.q0 + tok) * a.q_token + (int64_t)(w.h * a.group + r % a.group) * a.q_head + c0;
 #pragma unroll
             for (int k = 0; k < D / 16; ++k) {
@@ -164,28 +170,39 @@ __device__ __forceinline__ void products(Shared<D>& sh, const Args& a, int cta, 
             const uint32_t kt = tc::smem_u32(sh.ring[stage][0]) + k_off, vt = tc::smem_u32(sh.ring[stage][1]) + v_off;
             const int key0 = j * FEW_KEYS + strip;
             if (key0 < w.s.kv) {
-                float s[2][4] = {};
+                float s[2][4] = {}, s2[2][4] = {};                         // two sums each, so that half as many products wait for one another
 #pragma unroll
-                for (int k = 0; k < D / 16; ++k) {
-                    uint32_t b[4];
-                    const int ch = (2 * k + kch) & 7;
-                    ldsm(b, kt + (k >> 2) * across + ((ch ^ (krow & 7)) << 4));
+                for (int k = 0; k < D / 16; k += 2) {
+                    uint32_t b[4], b2[4];
+                    const uint32_t from = kt + (k >> 2) * across;
+                    ldsm(b, from ^ ((k & 3) << 5));
+                    ldsm(b2, from ^ (((k + 1) & 3) << 5));
                     mma<F16>(s[0], qf[k], b[0], b[1]);
                     mma<F16>(s[1], qf[k], b[2], b[3]);
+                    mma<F16>(s2[0], qf[k + 1], b2[0], b2[1]);
+                    mma<F16>(s2[1], qf[k + 1], b2[2], b2[3]);
                 }
-                float now[2] = {top[0], top[1]};
+                float now[2] = {-INFINITY, -INFINITY};
 #pragma unroll
                 for (int t = 0; t < 2; ++t)
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        const int key = key0 + 8 * t + c0 + (e & 1);
-                        s[t][e] = key < limit[e >> 1] ? s[t][e] * a.scale_log2 : -INFINITY;
-                        now[e >> 1] = fmaxf(now[e >> 1], s[t][e]);
-                    }
+                    for (int e = 0; e < 4; ++e) s[t][e] += s2[t][e];
+                if (__any_sync(0xffffffffu, min(limit[0], limit[1]) < key0 + 16)) {
+#pragma unroll
+                    for (int t = 0; t < 2; ++t)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e)
+                            if (key0 + 8 * t + c0 + (e & 1) >= limit[e >> 1]) s[t][e] = -INFINITY;
+                }
+#pragma unroll
+                for (int t = 0; t < 2; ++t)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) now[e >> 1] = fmaxf(now[e >> 1], s[t][e]);
 #pragma unroll
                 for (int i = 0; i < 2; ++i) {
                     now[i] = fmaxf(now[i], __shfl_xor_sync(0xffffffffu, now[i], 1));
                     now[i] = fmaxf(now[i], __shfl_xor_sync(0xffffffffu, now[i], 2));
+                    now[i] = fmaxf(now[i] * a.scale_log2, top[i]);
                 }
                 if (__any_sync(0xffffffffu, now[0] != top[0] || now[1] != top[1])) {
 #pragma unroll
@@ -200,28 +217,35 @@ __device__ __forceinline__ void products(Shared<D>& sh, const Args& a, int cta, 
                         top[i] = now[i];
                     }
                 }
-                const float base[2] = {top[0] == -INFINITY ? 0.f : top[0], top[1] == -INFINITY ? 0.f : top[1]};
+                const float base[2] = {top[0] == -INFINITY ? 0.f : -top[0], top[1] == -INFINITY ? 0.f : -top[1]};
 #pragma unroll
                 for (int t = 0; t < 2; ++t)
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {
-                        s[t][e] = ex2(s[t][e] - base[e >> 1]);
+                        s[t][e] = ex2(fmaf(s[t][e], a.scale_log2, base[e >> 1]));
                         total[e >> 1] += s[t][e];
                     }
                 const uint32_t p[4] = {pack2(s[0][0], s[0][1], F16), pack2(s[0][2], s[0][3], F16), pack2(s[1][0], s[1][1], F16),
                                        pack2(s[1][2], s[1][3], F16)};
-                // what lies behind the sequence is anything, also NaN, which no weight of zero takes away
-                const int past = key0 + 16 - w.s.kv;
-                const int k0 = key0 + c0;
-                const uint32_t m0 = past <= 0 ? 0xffffffffu : (k0 < w.s.kv ? 0xffffu : 0u) | (k0 + 1 < w.s.kv ? 0xffff0000u : 0u);
-                const uint32_t m1 = past <= 0 ? 0xffffffffu : (k0 + 8 < w.s.kv ? 0xffffu : 0u) | (k0 + 9 < w.s.kv ? 0xffff0000u : 0u);
+                auto add = [&](auto masked, uint32_t m0, uint32_t m1) {
 #pragma unroll
-                for (int d = 0; d < D / 16; ++d) {
-                    uint32_t b[4];
-                    const int ch = (2 * d + vch) & 7;
-                    ldsm_t(b, vt + (d >> 2) * across + ((ch ^ (vrow & 7)) << 4));
-                    mma<F16>(o[2 * d], p, b[0] & m0, b[1] & m1);
-                    mma<F16>(o[2 * d + 1], p, b[2] & m0, b[3] & m1);
+                    for (int d = 0; d < D / 16; ++d) {
+                        uint32_t b[4];
+                        ldsm_t(b, (vt + (d >> 2) * across) ^ ((d & 3) << 5));
+                        if constexpr (decltype(masked)::value) {
+                            b[0] &= m0, b[2] &= m0;
+                            b[1] &= m1, b[3] &= m1;
+                        }
+                        mma<F16>(o[2 * d], p, b[0], b[1]);
+                        mma<F16>(o[2 * d + 1], p, b[2], b[3]);
+                    }
+                };
+                if (key0 + 16 <= w.s.kv) add(std::false_type{}, 0u, 0u);
+                else {
+                    // what lies behind the sequence is anything, also NaN, which no weight of zero takes away
+                    const int k0 = key0 + c0;
+                    add(std::true_type{}, (k0 < w.s.kv ? 0xffffu : 0u) | (k0 + 1 < w.s.kv ? 0xffff0000u : 0u),
+                        (k0 + 8 < w.s.kv ? 0xffffu : 0u) | (k0 + 9 < w.s.kv ? 0xffff0000u : 0u));
                 }
             }
             __syncwarp();
