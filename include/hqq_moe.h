@@ -383,13 +383,14 @@ int hqm_rope_append_paged(const hqm_paged_append* a, void* stream);
  * cu_seqlens[b + 1] - 1 of q (tokens, n_heads, head_dim) and of out (contiguous).  With n of them and L positions in all, new
  * token i sees positions 0 .. L - n + i; n_heads / n_kv_heads (up to 128) query heads share a key/value head.  A row that sees nothing
  * (L - n + i < 0) is 0; rows behind the last sequence are left as they were.  Maximum, total and sums are fp32, the weights
- * are rounded to dtype for the product with v.  What pages hold behind a sequence may be anything, NaN included; inside a
- * sequence a value that is not finite may reach every row of the sequence.
+ * are rounded to dtype for the product with v.  What pages hold behind a sequence may be anything, NaN included.  A key that is
+ * not finite reaches the rows that see it (a score of NaN or +infinity makes the row NaN); a value that is not finite may reach every
+ * row of its sequence.
  *   hqm_paged_attention: k and v are pages, L = kv_lens[b] (the new tokens' keys and values are in the pages already);
  *     page_size 16 or more.  An entry of block_table outside the pool reads as zeros.
  *   hqm_prompt_attention: k and v (tokens, n_kv_heads, head_dim) lie like q, L = n; block_table, kv_lens and what describes
  *     pages are not used.
- * max_new: no sequence has more new tokens than this.  Nothing about lengths is read on the host, so a captured call follows
+ * max_new: no sequence has more new tokens than this (0: nothing is done).  Nothing about lengths is read on the host, so a captured call follows
  * them.  head_dim 64 or 128, scale positive; strides in elements, multiples of 8, rows 16-byte aligned.  scratch: any 16-byte aligned memory
  * of hqm_attention_scratch_bytes bytes that no other call in flight uses (nothing in it has to be initialised). */
 typedef struct hqm_attention {

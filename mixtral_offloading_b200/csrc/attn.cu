@@ -68,7 +68,7 @@ int check(const hqm_attention* c, bool paged, const char* what) {
                           c->v_page >= page_elements,
                       "%s: %d pages of %d positions (a power of two, 16 or more), %lld and %lld elements apart, rows of %d pages", what, c->pages,
                       c->page_size, (long long)c->k_page, (long long)c->v_page, c->max_pages);
-        HQM_CHECK_ARG((int64_t)c->max_pages * c->page_size <= INT32_MAX, "%s: rows of %d pages of %d positions", what, c->max_pages, c->page_size);
+        HQM_CHECK_ARG((int64_t)c->max_pages * c->page_size <= INT32_MAX - TILE_KEYS, "%s: rows of %d pages of %d positions", what, c->max_pages, c->page_size);
     }
     if (c->tokens == 0 || c->sequences == 0 || c->max_new == 0) return HQM_OK;
     HQM_CHECK_ARG(c->out && c->q && c->k && c->v && c->cu_seqlens && (!paged || (c->block_table && c->kv_lens)), "%s: null pointer", what);
@@ -194,7 +194,7 @@ extern "C" {
 
 size_t hqm_attention_scratch_bytes(const hqm_attention* c) {
     using namespace hqm::attn;
-    if (!c || c->n_kv_heads <= 0 || c->n_heads < c->n_kv_heads) return 0;
+    if (!c || c->n_kv_heads <= 0 || c->n_heads < c->n_kv_heads || (c->head_dim != 64 && c->head_dim != 128)) return 0;
     const int ctas = sm_count() > 0 ? sm_count() : 148;
     const Kernels k = Kernels::of(c, c->block_table != nullptr);
     return (k.tiles ? launch_bytes(ctas, TILE_ROWS, c->head_dim) : 0) + (k.few ? launch_bytes(ctas, FEW_TILE, c->head_dim) : 0);

@@ -298,6 +298,9 @@ class PagedDecode:
     def __init__(self, model: MixtralDecodeModel, sequences: int, pages: int, page_size: int = 64, max_len: Optional[int] = None):
         a0 = model.layers[0].attention
         dev = model.embed.device
+        if sequences < 1 or pages < 1 or page_size < 16 or page_size & (page_size - 1) or (max_len is not None and max_len < 1):
+            raise ValueError(f"{sequences} sequences of up to {max_len} positions, {pages} pages of {page_size}: pages are 16 positions or a larger "
+                             "power of two")
         self.model, self.page_size, self.pages = model, page_size, pages
         self.max_len = pages * page_size if max_len is None else max_len
         shape = (pages, a0.n_kv_heads, page_size, a0.head_dim)
@@ -326,12 +329,15 @@ class PagedDecode:
         after = [a + b for a, b in zip(self.lens, new)]
         if sum(new) == 0:
             raise ValueError("a step without tokens")
+        fed = [int(t) for ts in new_tokens for t in ts]
+        if not 0 <= min(fed) <= max(fed) < self.model.embed.shape[0]:
+            raise ValueError(f"tokens {min(fed)} .. {max(fed)}, the vocabulary has {self.model.embed.shape[0]}")
         if max(after) > self.max_len or self._pages(after) > self.pages:
             raise ValueError(f"{sum(new)} new tokens do not fit: {self._pages(after)} of {self.pages} pages, the longest sequence "
                              f"{max(after)} of {self.max_len}")
         T, most = sum(new), max(new)
         ends = [e - 1 for e, n in zip(itertools.accumulate(new), new) if n]
-        ids = self._to_device([int(t) for ts in new_tokens for t in ts], torch.int64)
+        ids = self._to_device(fed, torch.int64)
         s = paged_reserve(self.block_table, self.kv_lens, self.free_pages, self.free_count, self._to_device(new, torch.int32), self.page_size, T)
         prompts = all(a == 0 for a, n in zip(self.lens, new) if n)    # nothing cached that they could see
         self.lens = after
@@ -363,26 +369,30 @@ class PagedDecode:
     def generate(self, prompts: Sequence[Sequence[int]], new_tokens: int, chunk: int = 512, eos_token_id=None) -> List[List[int]]:
         """Greedy continuations of the prompts, one per sequence from the first on; prompts longer than `chunk` go in chunks, beside the
         tokens of those that are generating already.  What the sequences held before is dropped, and so is what they
-        hold in the end."""
+        hold in the end, also where the pool runs out in between (ValueError)."""
         if not 0 < len(prompts) <= len(self.lens) or any(len(p) == 0 for p in prompts) or chunk < 1 or new_tokens < 1:
             raise ValueError(f"up to {len(self.lens)} prompts of one token and more")
         self.truncate([0] * len(self.lens))
         feed = [list(p) for p in prompts] + [[] for _ in self.lens[len(prompts):]]
         out: List[List[int]] = [[] for _ in prompts]
-        while any(feed):
-            step = [f[:chunk] for f in feed]
-            feed = [f[chunk:] for f in feed]
-            logits = self.step(step)
-            fed = [b for b, f in enumerate(step) if f]
-            keep = list(self.lens)
-            for b, token in zip(fed, logits.argmax(-1).tolist()):
-                if feed[b]:
-                    continue                                          # in the middle of its prompt
-                out[b].append(token)
-                if len(out[b]) < new_tokens and token != eos_token_id:
-                    feed[b] = [token]
-                else:
-                    keep[b] = 0
-            if keep != self.lens:
-                self.truncate(keep)
+        try:
+            while any(feed):
+                step = [f[:chunk] for f in feed]
+                feed = [f[chunk:] for f in feed]
+                logits = self.step(step)
+                fed = [b for b, f in enumerate(step) if f]
+                keep = list(self.lens)
+                for b, token in zip(fed, logits.argmax(-1).tolist()):
+                    if feed[b]:
+                        continue                                          # in the middle of its prompt
+                    out[b].append(token)
+                    if len(out[b]) < new_tokens and token != eos_token_id:
+                        feed[b] = [token]
+                    else:
+                        keep[b] = 0
+                if keep != self.lens:
+                    self.truncate(keep)
+        finally:
+            if any(self.lens):
+                self.truncate([0] * len(self.lens))
         return out

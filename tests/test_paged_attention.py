@@ -220,6 +220,56 @@ def test_large_scores_and_a_peaked_softmax():
         check(p.paged(), *p.want(), what=str(order))
 
 
+@pytest.mark.parametrize("new", [1, 3, 90])
+@pytest.mark.parametrize("D,dtype", [(128, torch.bfloat16), (64, torch.float16)])
+def test_a_key_that_is_not_finite_reaches_the_rows_that_see_it(new, D, dtype):
+    """Every column of a block of keys in turn; rows that do not see it, and the other sequence, are as without it."""
+    L, group = 200, 4
+    for value in (float("nan"), float("inf"), -float("inf")):
+        for at in list(range(L - new - 1 if new > 1 else 100, L, 7)) + [L - 1, 0]:
+            p = Problem([L, 150], [new, new], 8, 2, D, 16, dtype, seed=at)
+            want, bound = p.want()
+            p.ks[0][at, :, 5] = value
+            refill(p.k_pages, p.table, p.ks, 16)
+            got = p.paged()
+            score = p.q[:new, :, 5].double() * value                   # NaN, or infinite with the sign of q
+            sees = torch.arange(new, device=DEV)[:, None] + L - new >= at
+            lost = sees & ~(score == -float("inf"))
+            assert torch.isnan(got[:new][lost]).all(), (value, at)
+            clean = torch.cat([~sees.expand(new, 8), torch.ones(new, 8, dtype=torch.bool, device=DEV)])
+            check(got[clean], want[clean], bound[clean], (value, at))
+            assert torch.isfinite(got[:new][~lost]).all()
+
+
+@pytest.mark.parametrize("D,dtype", [(128, torch.bfloat16), (64, torch.float16)])
+def test_the_largest_values_in_masked_places(D, dtype):
+    """Weights of masked places are exactly 0: values as large as the type has, in a later position, leave a row as it is."""
+    for new in (4, 90):
+        p = Problem([300, 40], [new, 2], 8, 2, D, 16, dtype)
+        want, bound = p.want()
+        p.vs[0][-1] = torch.finfo(dtype).max
+        p.ks[0][-1] = torch.finfo(dtype).max * 2.0 ** -12              # (finite scores)
+        refill(p.v_pages, p.table, p.vs, 16)
+        refill(p.k_pages, p.table, p.ks, 16)
+        got = p.paged()
+        rows = list(range(new - 1)) + [new, new + 1]
+        check(got[rows], want[rows], bound[rows], new)
+
+
+@pytest.mark.parametrize("pages", [1, 3, 5, 6, 40])
+@pytest.mark.parametrize("H,n_kv,D", [(32, 8, 128), (9, 3, 64), (4, 4, 128)])
+def test_tables_of_few_pages(pages, H, n_kv, D):
+    """Rows of the table from one block on: units that are not cut, and the same ones cut where the table is wide."""
+    page = 64
+    lens = [pages * page, pages * page - 5, 1]
+    for new in (1, 40):
+        p = Problem(lens, [min(new, L) for L in lens], H, n_kv, D, page, torch.bfloat16, seed=pages)
+        p.table = p.table[:, :pages].contiguous()
+        check(p.paged(), *p.want(), what=(pages, new))
+        wide = torch.cat([p.table, p.table.new_full((3, 50), -1)], 1)
+        check(paged_attention(p.q, p.k_pages, p.v_pages, wide, p.cu_seqlens, p.kv_lens, p.max_new), *p.want(), what="wide")
+
+
 def test_a_row_of_equal_scores():
     """q = 0: the mean of what a row sees, whatever the keys are; -3e38 as the keys' lowest values does not matter."""
     p = Problem([333, 140], [60, 1], 8, 2, 128, 16, torch.bfloat16)
@@ -287,6 +337,34 @@ def test_single_tokens_beside_chunks(H, n_kv, D, dtype):
     lens = [n + (37 * i) % 700 for i, n in enumerate(new)]
     p = Problem(lens, new, H, n_kv, D, 16, dtype)
     check(p.paged(), *p.want())
+
+
+def test_one_kind_of_sequences_alone_and_a_captured_call_of_both():
+    """A call made for both kinds of sequences that has only one of them, by its lengths or in a replay."""
+    p = Problem([700, 9, 40], [300, 5, 5], 32, 8, 128, 16, torch.bfloat16)                # all of many rows
+    check(p.paged(), *p.want(), what="many")
+    p = Problem([700, 300, 40, 90], [200, 1, 2, 1], 32, 8, 128, 16, torch.bfloat16)
+    out = torch.zeros_like(p.q)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        p.paged(out=out)
+    torch.cuda.current_stream().wait_stream(side)
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        p.paged(out=out)
+    for new in ([200, 1, 2, 1], [0, 1, 2, 1], [200, 0, 0, 0], [100, 100, 0, 4], [0, 0, 0, 0], [1, 200, 1, 1]):
+        lens = [max(n, L) for n, L in zip(new, (700, 300, 40, 90))]
+        lens = [min(L, k.shape[0]) for L, k in zip(lens, p.ks)]
+        cu = list(itertools.accumulate(new, initial=0))
+        p.cu_seqlens.copy_(torch.tensor(cu, dtype=torch.int32))
+        p.kv_lens.copy_(torch.tensor(lens, dtype=torch.int32))
+        out.fill_(2.5)
+        g.replay()
+        torch.cuda.synchronize()
+        want, bound = reference(p.q, [k[:L] for k, L in zip(p.ks, lens)], [v[:L] for v, L in zip(p.vs, lens)], cu, 128 ** -0.5)
+        check(out[:cu[-1]], want[:cu[-1]], bound[:cu[-1]], new)
+        assert (out[cu[-1]:] == 2.5).all()
 
 
 def test_max_new_is_a_bound_only():

@@ -102,3 +102,22 @@ def test_what_does_not_fit_is_refused(model):
         with pytest.raises(ValueError):
             p.generate(bad, 3)
     assert p.lens == [40, 16] == p.kv_lens.tolist()
+
+
+def test_shapes_and_tokens_that_cannot_be_are_refused(model):
+    for bad in ((0, 4, 16, 50), (2, 0, 16, 50), (2, 4, 8, 50), (2, 4, 48, 50), (2, 4, 16, 0)):
+        with pytest.raises(ValueError):
+            PagedDecode(model, *bad)
+    p = PagedDecode(model, 2, 4, 16, 50)
+    for bad in (-1, VOCAB):
+        with pytest.raises(ValueError):
+            p.step([[1, bad], []])
+    assert p.lens == [0, 0] == p.kv_lens.tolist() and p.free_count.item() == 4
+
+
+def test_a_pool_that_runs_out_is_empty_again(model):
+    p = PagedDecode(model, 2, 4, 16, 50)
+    with pytest.raises(ValueError):
+        p.generate([tokens(30, 1), tokens(31, 2)], 8)
+    assert p.lens == [0, 0] == p.kv_lens.tolist() and p.free_count.item() == 4
+    assert [len(o) for o in p.generate([tokens(3, 1), tokens(5, 2)], 4)] == [4, 4]
