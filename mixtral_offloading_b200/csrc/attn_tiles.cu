@@ -10,9 +10,17 @@
 //
 // S does not wait for the weights of the block before: it has columns of its own, and they are free as soon as the tile's warps
 // have S in registers.  With D = 64 both tiles have their own, with D = 128 there is room for one S (128 columns of S, 64 of p
-// per tile, 128 of O per tile: 512), which the tiles take in turns; each needs it for some 900 of the 2600 cycles that a block's
+// per tile, 128 of O per tile: 512), which the tiles take in turns; each needs it for some 900 of the 3000 cycles that a block's
 // weights take.  So the warps that form weights, which set the time, find the next S when they are done with one; where S lay under p
-// they waited for both products of their tile in every block, a third of the time (16001 tokens, 32 on 8 heads of 128: 1.91 ms).
+// they waited for both products of their tile in every block, a third of the time.
+//
+// Bound by the warps that form weights (two per scheduler, 32 x 128 of them in 3000 cycles: 1024 of the special-function unit, 400
+// instructions, the latencies between) and, with D = 128, nearly as much by the products: 8000 tokens, 32 on 8 heads, 0.43 ms with 128
+// columns (tensor cores 68 %, special-function unit 67 % busy) and 0.42 with 64 (39 %, 67 %).  16001 tokens of 128 columns: 1.84 ms = 1.14
+// PFLOP/s, 0.69 of the measured rate of products and 0.82 of the one under the power limit.  Tried and not kept: a part of the
+// exponentials by a polynomial on the other units (in this form no gain: 136 us become 146 for 24 packed prompts), 16 warps of half rows,
+// blocks of 64 positions, weights formed ahead of their maximum, one warp for both kinds of products (its waits and the
+// issues in turn: 2.3 ms), the results of a unit written behind the next one's first weights (5 % slower: registers).
 //
 // Warps 0-3: weights of tile 0, 4-7: of tile 1, 8: issues the products for S, 11: those for O (an issue takes as long as the product, so
 // that one warp for both would leave the tensor cores idle whenever it waits), 9: copies K and V of every block through a ring of
