@@ -133,6 +133,7 @@ struct Run {
 // Cost of the whole list.  Called by one whole warp.
 __device__ inline int64_t total_cost(const Args& a, const Cut& c) {
     int64_t total = 0;
+#pragma unroll 1
     for (int b = threadIdx.x & 31; b < a.B; b += 32) {
         const Seq s = load_seq(a, b, c);
         total += s.prefix(c, s.tiles);
@@ -146,33 +147,43 @@ __device__ inline int64_t total_cost(const Args& a, const Cut& c) {
 __device__ inline Run find_run(const Args& a, const Cut& c, int cta, int ctas) {
     const int lane = threadIdx.x & 31;
     auto cost = [&](const Seq& s) { return s.prefix(c, s.tiles) * a.n_kv; };
-    // the sequences one round of 32 after another; `sum` of a lane: the cost up to its sequence, within the round
-    Seq mine{};
-    int64_t w = 0, sum = 0;
-    auto round = [&](int b0) {
-        mine = Seq{};
-        if (b0 + lane < a.B) mine = load_seq(a, b0 + lane, c);
-        sum = w = cost(mine);
+    auto upto = [&](int64_t w) {                               // sum over the lanes up to this one
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
-            const int64_t v = __shfl_up_sync(0xffffffffu, sum, o);
-            if (lane >= o) sum += v;
+            const int64_t v = __shfl_up_sync(0xffffffffu, w, o);
+            if (lane >= o) w += v;
         }
+        return w;
     };
-    int64_t total = 0;
-    for (int b0 = 0; b0 < a.B; b0 += 32) {
-        round(b0);
-        total += __shfl_sync(0xffffffffu, sum, 31);
+    // a lane's share of the sequences, in one stretch; then the stretch that the run begins in, a sequence per lane
+    const int stretch = (a.B + 31) / 32;
+    Seq mine{};
+    int64_t w = 0;
+#pragma unroll 1
+    for (int i = 0; i < stretch; ++i) {
+        const int b = lane * stretch + i;
+        if (b >= a.B) break;
+        mine = load_seq(a, b, c);
+        w += cost(mine);
     }
+    int64_t sum = upto(w);
+    const int64_t total = __shfl_sync(0xffffffffu, sum, 31);
     Run r;
     r.share = quotient(total + ctas - 1, ctas);
     const int64_t lo = r.share * cta;
     r.left = min(max(total - lo, (int64_t)0), r.share);
     r.b = r.h = r.tile = r.skip = 0;
     if (r.left == 0) return r;
-    int64_t base = 0;
-    for (int b0 = 0; b0 < a.B; b0 += 32) {
-        if (a.B > 32) round(b0);                               // (else this one was the last)
+    const int owner = __ffs(__ballot_sync(0xffffffffu, sum > lo)) - 1;
+    int64_t base = stretch == 1 ? 0 : __shfl_sync(0xffffffffu, sum - w, owner);
+    const int from = stretch == 1 ? 0 : owner * stretch, to = stretch == 1 ? a.B : min(from + stretch, a.B);
+    for (int b0 = from; b0 < to; b0 += 32) {
+        if (stretch > 1) {
+            mine = Seq{};
+            if (b0 + lane < to) mine = load_seq(a, b0 + lane, c);
+            w = cost(mine);
+            sum = upto(w);
+        }
         const uint32_t past = __ballot_sync(0xffffffffu, base + sum > lo);
         if (past) {
             const int src = __ffs(past) - 1;

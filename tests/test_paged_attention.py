@@ -328,6 +328,20 @@ def test_many_sequences():
     check(p.paged(), *p.want())
 
 
+@pytest.mark.parametrize("B", [31, 32, 33, 64, 65, 100, 1100])
+def test_numbers_of_sequences(B):
+    """Around the 32 that a warp looks at at once; empty sequences, single tokens, a few and many rows."""
+    gen = torch.Generator().manual_seed(B)
+    lens = torch.randint(0, 200, (B,), generator=gen).tolist()
+    for most in (1, 30):
+        new = [min(L, int(n)) for L, n in zip(lens, torch.randint(0, most + 1, (B,), generator=gen))]
+        p = Problem(lens, new, 8, 2, 64, 16, torch.bfloat16, seed=B)
+        check(p.paged(), *p.want(), what=(B, most))
+    one = [0] * (B - 1) + [150]                                            # all of it in the last sequence
+    p = Problem([max(L, 1) for L in lens[:-1]] + [190], one, 8, 2, 64, 16, torch.bfloat16, seed=B)
+    check(p.paged(), *p.want(), what="last")
+
+
 @pytest.mark.parametrize("H,n_kv,D,dtype", [(32, 8, 128, torch.bfloat16), (16, 1, 64, torch.float16), (12, 2, 128, torch.float16)])
 def test_single_tokens_beside_chunks(H, n_kv, D, dtype):
     """Sequences of up to 16 rows per key/value head and longer ones in one call, around that line, empty ones among them."""
