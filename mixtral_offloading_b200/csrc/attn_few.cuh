@@ -31,7 +31,8 @@ struct Shared {
     static constexpr int HALVES = D / 64;
     static constexpr int TILE = FEW_KEYS * 128 * HALVES;          // 64 positions: boxes of [64 columns][rows of a box][128 bytes], 128-byte swizzle
     alignas(1024) unsigned char ring[STAGES][2][TILE];            // K, V
-    float sums[CONSUMERS][FEW_TILE][D];
+    static constexpr int PITCH = D + 8;                           // four rows of a quad's eight columns on banks of their own
+    float sums[CONSUMERS][FEW_TILE][PITCH];
     float top[CONSUMERS][FEW_TILE], total[CONSUMERS][FEW_TILE];
     uint64_t full[STAGES], empty[STAGES];
     Run run;
@@ -145,6 +146,15 @@ __device__ __forceinline__ void products(Shared<D>& sh, const Args& a, int cta, 
     const int krow = strip + (lane & 7) + ((lane >> 4) << 3), kch = (lane >> 3) & 1, vrow = strip + (lane & 15), vch = lane >> 4;
     // (16-byte columns of a row lie at their number xor the row's: those of step k at the first step's address xor 32 k)
     const uint32_t k_off = key_at(krow) + ((kch ^ (krow & 7)) << 4), v_off = key_at(vrow) + ((vch ^ (vrow & 7)) << 4);
+    int tok[2];                                                            // of the two rows: token within the unit, where its q lies
+    int64_t q_at[2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        tok[i] = (r0 + 8 * i) / a.group;
+        q_at[i] = tok[i] * a.q_token + (r0 + 8 * i - tok[i] * a.group) * a.q_head + c0;
+    }
+    // of the row that this thread writes results of, the first of its n_rows * D / 2 / threads
+    const int out_row = threadIdx.x / (D / 2), out_step = 32 * CONSUMERS / (D / 2);
     uint32_t at = 0;
     bool split = false;
     while (w.next()) {
@@ -153,14 +163,16 @@ __device__ __forceinline__ void products(Shared<D>& sh, const Args& a, int cta, 
         int limit[2];                                                      // positions that the two rows see
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
-            const int r = r0 + 8 * i, tok = tok0 + r / a.group;
-            limit[i] = r < n_rows ? w.s.before + tok + 1 : w.s.kv;              // (a row of padding is nobody's)
-            const uint16_t* src = a.q + (int64_t)(w.s.q0 + tok) * a.q_token + (int64_t)(w.h * a.group + r % a.group) * a.q_head + c0;
+            const bool valid = r0 + 8 * i < n_rows;
+            limit[i] = valid ? w.s.before + tok0 + tok[i] + 1 : w.s.kv;    // (a row of padding is nobody's)
+            const uint16_t* src = a.q + (int64_t)(w.s.q0 + tok0) * a.q_token + (int64_t)(w.h * a.group) * a.q_head + q_at[i];
 #pragma unroll
             for (int k = 0; k < D / 16; ++k) {
-                qf[k][i] = r < n_rows ? *reinterpret_cast<const uint32_t*>(src + 16 * k) : 0u;
-                qf[k][i + 2] = r < n_rows ? *reinterpret_cast<const uint32_t*>(src + 16 * k + 8) : 0u;
+                qf[k][i] = valid ? *reinterpret_cast<const uint32_t*>(src + 16 * k) : 0u;
+                qf[k][i + 2] = valid ? *reinterpret_cast<const uint32_t*>(src + 16 * k + 8) : 0u;
             }
+            if (valid && w.h + 1 < a.n_kv && (lane & 3) < D / 64)          // the next unit's, most of the time
+                asm volatile("prefetch.global.L1 [%0];" ::"l"(src + a.group * a.q_head + (lane & 3) * 64));
         }
         float o[D / 8][4];
 #pragma unroll
@@ -275,8 +287,9 @@ __device__ __forceinline__ void products(Shared<D>& sh, const Args& a, int cta, 
         sync_consumers();
         const bool whole = w.whole();
         float* piece = whole ? nullptr : piece_at<D>(a, cta, w.j0 == 0);
-        for (int i = threadIdx.x; i < n_rows * (D / 2); i += 32 * CONSUMERS) {
-            const int r = i / (D / 2), d = (i % (D / 2)) * 2;
+        const int64_t row0 = (int64_t)(w.s.q0 + tok0) * (a.n_kv * a.group) + w.h * a.group;
+        for (int r = out_row; r < n_rows; r += out_step) {
+            const int d = threadIdx.x % (D / 2) * 2;
             float m = -INFINITY;
 #pragma unroll
             for (int k = 0; k < CONSUMERS; ++k) m = fmaxf(m, sh.top[k][r]);
@@ -291,7 +304,7 @@ __device__ __forceinline__ void products(Shared<D>& sh, const Args& a, int cta, 
             }
             if (whole) {
                 const float inv = m == -INFINITY ? 0.f : 1.f / l;
-                const int64_t row = (int64_t)(w.s.q0 + tok0 + r / a.group) * (a.n_kv * a.group) + w.h * a.group + r % a.group;
+                const int64_t row = row0 + r + (n_rows > a.group ? r / a.group * (a.n_kv - 1) * a.group : 0);
                 *reinterpret_cast<uint32_t*>(a.out + row * D + d) = pack2(x * inv, y * inv, F16);
             } else {
                 *reinterpret_cast<float2*>(piece + r * D + d) = make_float2(x, y);
