@@ -274,6 +274,24 @@ def test_the_library_refuses_what_it_cannot_do():
     assert lib.hqm_paged_truncate(some, 8, some, some, None, some, some, 4, 8, 16, 100, None) == _cabi.HQM_ERR_ARG
 
 
+def test_a_result_that_shares_memory_with_what_is_read_is_refused():
+    lib = _cabi.lib()
+    ok = dict(q=1 << 20, k=2 << 20, v=3 << 20, q_token=512, q_head=128, k_token=256, k_head=128, v_token=256, v_head=128, k_page=4096, v_page=4096,
+              block_table=4096, table_stride=4, cu_seqlens=4096, kv_lens=4096, tokens=3, sequences=1, max_new=3, n_heads=4, n_kv_heads=2,
+              head_dim=128, pages=9, page_size=16, max_pages=4, dtype=0, scale=0.1)
+    size = 3 * 512 * 2
+    for out in (1 << 20, (1 << 20) + size - 16, (1 << 20) - size + 16):
+        for entry in (lib.hqm_paged_attention, lib.hqm_prompt_attention):
+            assert entry(C.byref(_cabi.HqmAttention(**dict(ok, out=out))), C.c_void_p(4096), 0, None) == _cabi.HQM_ERR_ARG
+            assert "shares memory" in _cabi.last_error()
+    for out in (2 << 20, (3 << 20) + 256):
+        assert lib.hqm_prompt_attention(C.byref(_cabi.HqmAttention(**dict(ok, out=out))), C.c_void_p(4096), 0, None) == _cabi.HQM_ERR_ARG
+        assert "shares memory" in _cabi.last_error()
+    # right behind q: refused for another reason (no scratch, or no device), not for its place
+    lib.hqm_paged_attention(C.byref(_cabi.HqmAttention(**dict(ok, out=(1 << 20) + size))), C.c_void_p(4096), 0, None)
+    assert "shares memory" not in _cabi.last_error()
+
+
 def test_no_cpu_path():
     t = torch.zeros(1, 4, 64, dtype=torch.bfloat16)
     i = torch.zeros(1, dtype=torch.int32)
