@@ -86,7 +86,10 @@ struct Seq {
     }
     // Cost of tiles 0 .. count - 1.  A tile that sees nothing has one block.  The others of `per` tokens, from tile `empty` on, have
     // floor((per i + b) / block): where both are powers of two the sum is that of an arithmetic progression in groups of equal terms.
+    // Nothing where the launch leaves the sequence out (tiles == 0), also where it has fewer positions than tokens: a walk passes it
+    // without a cost, and runs that did not agree with that would leave blocks to nobody.
     __host__ __device__ int64_t prefix(const Cut& c, int count) const {
+        if (tiles == 0) return 0;
         const int whole = min(count, tiles - 1);               // tiles of `per` tokens
         int empty = 0;
         if (before < 0) empty = min(whole, -before / c.per);
@@ -103,12 +106,12 @@ struct Seq {
                 sum += upto(first + n) - upto(first);
             }
         }
-        if (count >= tiles && tiles > 0) sum += blocks(c, tiles - 1);
+        if (count >= tiles) sum += blocks(c, tiles - 1);
         return sum;
     }
 };
 
-__device__ __forceinline__ Seq load_seq(const Args& a, int b, const Cut& c) {
+__host__ __device__ __forceinline__ Seq load_seq(const Args& a, int b, const Cut& c) {
     Seq s;
     const int lo = min(max(a.cu[b], 0), a.T), hi = min(max(a.cu[b + 1], lo), a.T);
     s.q0 = lo;
@@ -227,8 +230,8 @@ struct Walk {
     int64_t left;
     int b, h, tile, skip;
     int j0, j1, blocks;            // the part: blocks j0 .. j1 - 1 of `blocks`
-    __device__ Walk(const Args& args, const Run& r, const Cut& c) : a(args), cut(c), s(r.s), left(r.left), b(r.b), h(r.h), tile(r.tile), skip(r.skip) {}
-    __device__ bool next() {       // false: done
+    __host__ __device__ Walk(const Args& args, const Run& r, const Cut& c) : a(args), cut(c), s(r.s), left(r.left), b(r.b), h(r.h), tile(r.tile), skip(r.skip) {}
+    __host__ __device__ bool next() {      // false: done
         while (left > 0) {
             if (tile == s.tiles) {
                 tile = 0;
@@ -258,9 +261,9 @@ struct Walk {
         return false;
     }
     // the part's tile is tile - 1 from here on
-    __device__ int first_token() const { return (tile - 1) * cut.per; }
-    __device__ int tokens() const { return min(cut.per, s.n - first_token()); }
-    __device__ bool whole() const { return j0 == 0 && j1 == blocks; }
+    __host__ __device__ int first_token() const { return (tile - 1) * cut.per; }
+    __host__ __device__ int tokens() const { return min(cut.per, s.n - first_token()); }
+    __host__ __device__ bool whole() const { return j0 == 0 && j1 == blocks; }
 };
 
 // A piece: sums, then maxima [rows] (base 2), then totals [rows].  The sums of attn_few.cu lie as [rows][D]; those of attn_tiles.cu, where
