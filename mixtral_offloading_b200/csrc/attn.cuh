@@ -316,6 +316,17 @@ int launch_tiles(const Args& a, const CUtensorMap& qm, const CUtensorMap& km, co
 int launch_mixed(const Args& a, const Args& f, const CUtensorMap& qm, const CUtensorMap& km, const CUtensorMap& vm, const CUtensorMap& kf,
                  const CUtensorMap& vf, int ctas, int D, bool f16, cudaStream_t st);
 
+// A ring of N buffers with a barrier for "copied" and one for "used" each; item i of a warp's list lies in buffer(i).  A barrier tells the
+// phase that it is in by its parity alone, so a warp that waits on one has to wait for every phase of it, one after another: for a
+// phase whose predecessor it has not seen a wait passes at once, on what lay there before.  Hence every warp that waits
+// on a ring takes all of its items.
+template <int N>
+struct Ring {
+    __host__ __device__ static int buffer(uint32_t i) { return (int)(i % N); }
+    __host__ __device__ static uint32_t copied(uint32_t i) { return (i / N) & 1; }             // parity of the phase in which item i arrives
+    __host__ __device__ static uint32_t used(uint32_t i) { return (i / N - 1) & 1; }           // in which the item in its place before was used, i >= N
+};
+
 constexpr int FEW_TILE = 16;       // rows of a unit of attn_few.cu
 constexpr int FEW_KEYS = 64, FEW_KEYS_LOG = 6;         // positions of a block there
 constexpr int TILE_ROWS = 256;     // rows of a unit of attn_tiles.cu

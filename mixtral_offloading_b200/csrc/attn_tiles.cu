@@ -23,8 +23,9 @@
 // issues in turn: 2.3 ms), the results of a unit written behind the next one's first weights (5 % slower: registers).
 //
 // Warps 0-3: weights of tile 0, 4-7: of tile 1, 8: issues the products for S, 11: those for O (an issue takes as long as the product, so
-// that one warp for both would leave the tensor cores idle whenever it waits), 9: copies K and V of every block through a ring of
-// five buffers (cp.async.bulk.tensor; of a paged cache a copy per page), 10: walks the list of units and copies their Q.
+// that one warp for both would leave the tensor cores idle whenever it waits), 9: copies K and V of every block through rings of
+// three and two buffers (cp.async.bulk.tensor; of a paged cache a copy per page), 10: walks the list of units and copies their Q.
+// K and V have rings of their own, since warp 8 waits for K only and warp 11 for V only (Ring).
 //
 // The maximum m that a row's weights refer to is raised only when a block exceeds it by more than 2^8: O, which lies in tensor
 // memory, is rescaled a few times per unit instead of once per block, weights grow to 256 at the most, and l and O mean the same
@@ -39,7 +40,9 @@ namespace attn {
 namespace {
 
 constexpr int KEYS = TILE_KEYS;
-constexpr int RING = 5;
+constexpr int K_RING = 3, V_RING = 2;
+typedef Ring<K_RING> KRing;
+typedef Ring<V_RING> VRing;
 // Three warpgroups of 168 registers a thread at the launch (64512): the two that form weights take 216, the third keeps 72.
 constexpr int WEIGHT_WARPS = 8, THREADS = 32 * WEIGHT_WARPS + 128;
 constexpr int REGS_WEIGHTS = 216, REGS_OTHERS = 72;
@@ -65,8 +68,9 @@ struct Shared {
     static constexpr int PANEL = 128 * 128;                       // 128 rows x 64 columns, 128-byte swizzle
     static constexpr int TILE = HALVES * PANEL;
     alignas(1024) unsigned char q[2][TILE];
-    alignas(1024) unsigned char ring[RING][TILE];                 // K, V, K, V, ...
-    uint64_t full[RING], empty[RING], q_full[2], q_empty[2], s_full[2], s_read[2], p_full[2], o_done[2];
+    alignas(1024) unsigned char k[K_RING][TILE], v[V_RING][TILE];
+    uint64_t k_full[K_RING], k_empty[K_RING], v_full[V_RING], v_empty[V_RING];
+    uint64_t q_full[2], q_empty[2], s_full[2], s_read[2], p_full[2], o_done[2];
     uint64_t part_full[PARTS], part_empty[PARTS];
     Part parts[PARTS];
     uint32_t tmem;
@@ -199,9 +203,13 @@ __device__ __forceinline__ void tiles_cta(Shared<D>& sh, const CUtensorMap& qm, 
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int per_tile = 128 / a.group;                            // tokens
     if (threadIdx.x == 0) {
-        for (int i = 0; i < RING; ++i) {
-            tc::mbar_init(&sh.full[i], 1);
-            tc::mbar_init(&sh.empty[i], 1);
+        for (int i = 0; i < K_RING; ++i) {
+            tc::mbar_init(&sh.k_full[i], 1);
+            tc::mbar_init(&sh.k_empty[i], 1);
+        }
+        for (int i = 0; i < V_RING; ++i) {
+            tc::mbar_init(&sh.v_full[i], 1);
+            tc::mbar_init(&sh.v_empty[i], 1);
         }
         for (int t = 0; t < 2; ++t) {
             tc::mbar_init(&sh.q_full[t], 1);
@@ -383,7 +391,7 @@ __device__ __forceinline__ void tiles_cta(Shared<D>& sh, const CUtensorMap& qm, 
             uint32_t at = 0;
             while (next()) {
                 const int32_t* table = a.table + (int64_t)w.table_row * a.table_stride;
-                for (int j = w.j0; j < w.j1; ++j) {
+                for (int j = w.j0; j < w.j1; ++j, ++at) {
                     const int key = j * KEYS + lane * rows;            // of box `lane`; there are eight at the most
                     const int live = min(boxes, (max(w.kv - j * KEYS, 0) + rows - 1) / rows);
                     int row = w.kv_row + key, page = 0;
@@ -391,34 +399,37 @@ __device__ __forceinline__ void tiles_cta(Shared<D>& sh, const CUtensorMap& qm, 
                         page = min((uint32_t)table[key >> a.page_shift], (uint32_t)a.n_pages);      // outside the pool: zeros
                         row = key & ((1 << a.page_shift) - 1);
                     }
-                    for (int kv = 0; kv < 2; ++kv, ++at) {
-                        const int slot = at % RING;
-                        if (at >= RING) patience.wait(&sh.empty[slot], (at / RING - 1) & 1);
+                    auto copy = [&](unsigned char* to, const CUtensorMap* map, uint64_t* full) {
                         patience.ok = __all_sync(0xffffffffu, patience.ok);
                         if (patience.ok) {
-                            if (lane == 0) expect(&sh.full[slot], (uint32_t)live * rows * 128 * S::HALVES);
+                            if (lane == 0) expect(full, (uint32_t)live * rows * 128 * S::HALVES);
                             __syncwarp();
                             if (lane < live)
 #pragma unroll
                                 for (int h = 0; h < S::HALVES; ++h)
-                                    copy_box(tc::smem_u32(sh.ring[slot] + h * S::PANEL + lane * rows * 128), kv ? &vm : &km, 64 * h, row, w.head, page,
-                                             &sh.full[slot]);
+                                    copy_box(tc::smem_u32(to + h * S::PANEL + lane * rows * 128), map, 64 * h, row, w.head, page, full);
                         }
                         __syncwarp();
-                    }
+                    };
+                    const int ks = KRing::buffer(at), vs = VRing::buffer(at);
+                    if (at >= K_RING) patience.wait(&sh.k_empty[ks], KRing::used(at));
+                    copy(sh.k[ks], &km, &sh.k_full[ks]);
+                    if (at >= V_RING) patience.wait(&sh.v_empty[vs], VRing::used(at));
+                    copy(sh.v[vs], &vm, &sh.v_full[vs]);
                 }
             }
             // no copy may be on its way when the CTA ends
             Patience last;
-            for (uint32_t k = at < RING ? 0 : at - RING; k < at; ++k) last.wait(&sh.full[k % RING], (k / RING) & 1);
+            for (uint32_t k = at < K_RING ? 0 : at - K_RING; k < at; ++k) last.wait(&sh.k_full[KRing::buffer(k)], KRing::copied(k));
+            for (uint32_t k = at < V_RING ? 0 : at - V_RING; k < at; ++k) last.wait(&sh.v_full[VRing::buffer(k)], VRing::copied(k));
         } else if (warp == WEIGHT_WARPS) {
             // ---- S = Q K^T ----
             const uint32_t idesc = (1u << 4) | (F16 ? 0u : (1u << 7) | (1u << 10)) | ((KEYS / 8) << 17) | ((128u >> 4) << 24);
             uint32_t at = 0, units[2] = {0, 0}, made[2] = {0, 0};
             while (next()) {
-                for (int j = w.j0; j < w.j1; ++j, at += 2) {
-                    const int slot = at % RING;
-                    patience.wait(&sh.full[slot], (at / RING) & 1);
+                for (int j = w.j0; j < w.j1; ++j, ++at) {
+                    const int slot = KRing::buffer(at);
+                    patience.wait(&sh.k_full[slot], KRing::copied(at));
 #pragma unroll
                     for (int t = 0; t < 2; ++t) {
                         const int end = t == 0 ? w.end0 : w.tokens > per_tile ? w.j1 : 0;
@@ -428,7 +439,7 @@ __device__ __forceinline__ void tiles_cta(Shared<D>& sh, const CUtensorMap& qm, 
                         if (made[buffer]++ > 0) patience.wait(&sh.s_read[buffer], made[buffer] & 1);       // (of the one before the last)
                         fence_after();
                         if (elected()) {
-                            const uint64_t qa = tc::smem_desc_sw128(tc::smem_u32(sh.q[t])), kb = tc::smem_desc_sw128(tc::smem_u32(sh.ring[slot]));
+                            const uint64_t qa = tc::smem_desc_sw128(tc::smem_u32(sh.q[t])), kb = tc::smem_desc_sw128(tc::smem_u32(sh.k[slot]));
 #pragma unroll
                             for (int k = 0; k < D / 16; ++k) {
                                 const uint64_t off = ((k >> 2) * S::PANEL + (k & 3) * 32) >> 4;
@@ -439,25 +450,25 @@ __device__ __forceinline__ void tiles_cta(Shared<D>& sh, const CUtensorMap& qm, 
                         }
                         __syncwarp();
                     }
-                    if (elected()) tc::umma_commit(&sh.empty[slot]);
+                    if (elected()) tc::umma_commit(&sh.k_empty[slot]);
                     __syncwarp();
                 }
             }
         } else if (warp == WEIGHT_WARPS + 3) {
             // ---- O += p V ----
             const uint32_t idesc = (1u << 4) | (F16 ? 0u : (1u << 7) | (1u << 10)) | (1u << 16) | ((D / 8) << 17) | ((128u >> 4) << 24);
-            uint32_t at = 1, used[2] = {0, 0};
+            uint32_t at = 0, used[2] = {0, 0};
             while (next()) {
-                for (int j = w.j0; j < w.j1; ++j, at += 2) {
-                    const int slot = at % RING;
-                    patience.wait(&sh.full[slot], (at / RING) & 1);
+                for (int j = w.j0; j < w.j1; ++j, ++at) {
+                    const int slot = VRing::buffer(at);
+                    patience.wait(&sh.v_full[slot], VRing::copied(at));
                     const int live = w.kv - j * KEYS;                      // positions of the block that belong to the sequence
                     if (live < KEYS) {
                         // behind them lies anything, also NaN, which no weight of zero takes away
                         for (int i = max(live, 0) * 8 + lane; i < KEYS * 8; i += 32)
 #pragma unroll
                             for (int h = 0; h < S::HALVES; ++h)
-                                *reinterpret_cast<uint4*>(sh.ring[slot] + h * S::PANEL + i * 16) = make_uint4(0, 0, 0, 0);
+                                *reinterpret_cast<uint4*>(sh.v[slot] + h * S::PANEL + i * 16) = make_uint4(0, 0, 0, 0);
                         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                         __syncwarp();
                     }
@@ -467,7 +478,7 @@ __device__ __forceinline__ void tiles_cta(Shared<D>& sh, const CUtensorMap& qm, 
                         patience.wait(&sh.p_full[t], used[t]++ & 1);
                         fence_after();
                         if (elected()) {
-                            const uint64_t vb = desc_across(tc::smem_u32(sh.ring[slot]), S::PANEL);
+                            const uint64_t vb = desc_across(tc::smem_u32(sh.v[slot]), S::PANEL);
 #pragma unroll
                             for (int k = 0; k < KEYS / 16; ++k)
                                 mma_ts(tmem + O_AT + D * t, tmem + P_AT + 64 * t + 8 * k, vb + ((k * 16 * 128) >> 4), idesc, j > w.j0 || k > 0);
@@ -475,7 +486,7 @@ __device__ __forceinline__ void tiles_cta(Shared<D>& sh, const CUtensorMap& qm, 
                         }
                         __syncwarp();
                     }
-                    if (elected()) tc::umma_commit(&sh.empty[slot]);
+                    if (elected()) tc::umma_commit(&sh.v_empty[slot]);
                     __syncwarp();
                 }
             }
