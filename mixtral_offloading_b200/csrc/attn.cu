@@ -132,6 +132,7 @@ int run(const hqm_attention* c, bool paged, const char* what, void* scratch, siz
     Args a{};
     a.q = (const uint16_t*)c->q;
     a.out = (uint16_t*)c->out;
+    a.out_32 = (reinterpret_cast<uintptr_t>(c->out) & 31u) == 0;
     a.q_token = c->q_token;
     a.q_head = c->q_head;
     a.table = paged ? c->block_table : nullptr;

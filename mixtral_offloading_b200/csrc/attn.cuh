@@ -22,6 +22,7 @@ namespace attn {
 struct Args {
     const uint16_t* q;
     uint16_t* out;                 // (T, n_heads, D), contiguous
+    int out_32;                    // whether out begins on a 32-byte boundary (a 16-byte one it does in any case)
     int64_t q_token, q_head;       // strides of q, in elements
     const int32_t* table;          // null: keys and values are packed like the queries
     int64_t table_stride;

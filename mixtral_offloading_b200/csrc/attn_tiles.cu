@@ -109,7 +109,8 @@ __device__ __forceinline__ void copy_box(uint32_t dst, const CUtensorMap* map, i
 __device__ __forceinline__ void fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
 
-// A lane's row lies in lines of its own, so that the stores of a warp take a cycle per lane and instruction: as wide as they come.
+// A lane's row lies in lines of its own, so that the stores of a warp take a cycle per lane and instruction: as wide as they come
+// where `out` allows it (Args::out_32), else half of that.
 __device__ __forceinline__ void store_32_bytes(void* at, const uint32_t* v) {
     asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(at), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]),
                  "r"(v[6]), "r"(v[7]) : "memory");
@@ -370,8 +371,13 @@ __device__ __forceinline__ void tiles_cta(Shared<D>& sh, const CUtensorMap& qm, 
                 if (whole) {
 #pragma unroll
                     for (int i = 0; i < 16; ++i) o[i] = pack2(__uint_as_float(o[2 * i]) * inv, __uint_as_float(o[2 * i + 1]) * inv, F16);
-                    store_32_bytes(a.out + row * D + c, o);
-                    store_32_bytes(a.out + row * D + c + 16, o + 8);
+                    if (a.out_32) {
+                        store_32_bytes(a.out + row * D + c, o);
+                        store_32_bytes(a.out + row * D + c + 16, o + 8);
+                    } else {
+#pragma unroll
+                        for (int i = 0; i < 16; i += 4) *reinterpret_cast<uint4*>(a.out + row * D + c + 2 * i) = make_uint4(o[i], o[i + 1], o[i + 2], o[i + 3]);
+                    }
                 } else {
 #pragma unroll
                     for (int i = 0; i < 32; i += 4)
