@@ -380,8 +380,8 @@ typedef struct hqm_paged_append {
 int hqm_rope_append_paged(const hqm_paged_append* a, void* stream);
 
 /* out = softmax(scale * q k^T) v for the new tokens of many sequences at once: sequence b's are rows cu_seqlens[b] ..
- * cu_seqlens[b + 1] - 1 of q (tokens, n_heads, head_dim) and of out (contiguous, no memory of q's).  With n of them and L positions in all, new
- * token i sees positions 0 .. L - n + i; n_heads / n_kv_heads (up to 128) query heads share a key/value head.  A row that sees nothing
+ * cu_seqlens[b + 1] - 1 of q (tokens, n_heads, head_dim) and of out (contiguous, none of the memory of q, k and v).  With n of them and L
+ * positions in all, new token i sees positions 0 .. L - n + i; n_heads / n_kv_heads (up to 128) query heads share a key/value head.  A row that sees nothing
  * (L - n + i < 0) is 0; rows behind the last sequence are left as they were.  Maximum, total and sums are fp32, the weights
  * are rounded to dtype for the product with v.  What pages hold behind a sequence may be anything, NaN included.  A key that is
  * not finite reaches the rows that see it (a score of NaN or +infinity makes the row NaN); a value that is not finite may reach every

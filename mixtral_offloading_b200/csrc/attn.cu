@@ -3,6 +3,7 @@
 #include <math.h>
 
 #include "attn.cuh"
+#include "overlap.h"
 
 namespace hqm {
 namespace attn {
@@ -50,11 +51,6 @@ bool encode_kv(CUtensorMap* to, const void* at, int D, int rows, cuuint64_t posi
     return encode(to, at, 4, dims, strides, box, f16);
 }
 
-// Whether (tokens, heads, D) at p, strides in elements, from its first element to its last, shares memory with the `elements` at out.
-bool meets(const void* out, int64_t elements, const void* p, int64_t tokens, int64_t heads, int64_t token, int64_t head, int64_t D) {
-    const uintptr_t o = reinterpret_cast<uintptr_t>(out), x = reinterpret_cast<uintptr_t>(p);
-    return x < o + 2 * elements && o < x + 2 * ((tokens - 1) * token + (heads - 1) * head + D);
-}
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 
 int check(const hqm_attention* c, bool paged, const char* what) {
@@ -81,12 +77,12 @@ int check(const hqm_attention* c, bool paged, const char* what) {
     HQM_CHECK_ARG(strides % 8 == 0 && aligned16(c->q) && aligned16(c->k) && aligned16(c->v) && aligned16(c->out),
                   "%s: rows have to start on 16-byte boundaries", what);
     if (!paged) HQM_CHECK_ARG(c->k_token > 0 && c->k_head > 0 && c->v_token > 0 && c->v_head > 0, "%s: strides of keys and values have to be positive", what);
-    // (a CTA may have written its rows of out before another one has read the same rows of q)
-    const int64_t all = c->tokens * c->n_heads * c->head_dim;
-    bool shared = meets(c->out, all, c->q, c->tokens, c->n_heads, c->q_token, c->q_head, c->head_dim);
-    if (!paged)
-        shared = shared || meets(c->out, all, c->k, c->tokens, c->n_kv_heads, c->k_token, c->k_head, c->head_dim) ||
-                 meets(c->out, all, c->v, c->tokens, c->n_kv_heads, c->v_token, c->v_head, c->head_dim);
+    const Stretch out = elements_at(c->out, c->tokens * c->n_heads * c->head_dim);
+    const int64_t page_elements = (int64_t)c->n_kv_heads * c->page_size * c->head_dim;
+    const bool shared = out.meets(rows_at(c->q, c->tokens, c->n_heads, c->q_token, c->q_head, c->head_dim)) ||
+                        (paged ? Pages{c->k, c->pages, c->k_page, page_elements}.meets(out) || Pages{c->v, c->pages, c->v_page, page_elements}.meets(out)
+                               : out.meets(rows_at(c->k, c->tokens, c->n_kv_heads, c->k_token, c->k_head, c->head_dim)) ||
+                                     out.meets(rows_at(c->v, c->tokens, c->n_kv_heads, c->v_token, c->v_head, c->head_dim)));
     HQM_CHECK_ARG(!shared, "%s: out shares memory with what is read", what);
     return HQM_OK;
 }
