@@ -362,7 +362,8 @@ int hqm_paged_truncate(const int32_t* block_table, int64_t table_stride, int32_t
  * hqm_rope_append_rows, which rounds to bf16 after every operation as Hugging Face does, angles are formed in 64 bits and a
  * result is rounded once.  q (tokens, n_heads, head_dim), k and v (tokens, n_kv_heads, head_dim), strides in elements,
  * multiples of 8, rows 16-byte aligned; q_out (tokens, n_heads, head_dim) contiguous, may be q.  k_out (NULL: not wanted): the
- * rotated k as well, (tokens, n_kv_heads, head_dim) contiguous, may be k; what hqm_prompt_attention wants.  A token whose slot is
+ * rotated k as well, (tokens, n_kv_heads, head_dim) contiguous, may be k; what hqm_prompt_attention wants.  Beyond that q_out, k_out, k_pages
+ * and v_pages share no memory with one another or with q, k and v (refused; between pages there may be others).  A token whose slot is
  * negative is left out (its rows of q_out and k_out stay); one beyond the pool is too, and makes hqm_device_error() return 2. */
 typedef struct hqm_paged_append {
     void *q_out, *k_out;

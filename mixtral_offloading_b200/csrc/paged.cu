@@ -15,6 +15,7 @@
 
 #include "common.cuh"
 #include "kernels.cuh"
+#include "overlap.h"
 #include "shared_limit.h"
 
 namespace hqm {
@@ -397,6 +398,20 @@ int hqm_rope_append_paged(const hqm_paged_append* a, void* stream) {
     HQM_CHECK_ARG(strides % 8 == 0 && aligned16(a->q_out) && aligned16(a->k_out) && aligned16(a->q) && aligned16(a->k) && aligned16(a->v) && aligned16(a->k_pages) &&
                       aligned16(a->v_pages),
                   "rope_append_paged: rows have to start on 16-byte boundaries");
+    // in place is safe, a thread reads what it is about to write; any other meeting is between threads
+    const Stretch q = rows_at(a->q, a->tokens, a->n_heads, a->q_token, a->q_head, a->head_dim), q_out = elements_at(a->q_out, a->tokens * a->n_heads * a->head_dim);
+    const Stretch k = rows_at(a->k, a->tokens, a->n_kv_heads, a->k_token, a->k_head, a->head_dim), v = rows_at(a->v, a->tokens, a->n_kv_heads, a->v_token, a->v_head, a->head_dim);
+    const Stretch k_out = elements_at(a->k_out, a->k_out ? a->tokens * a->n_kv_heads * a->head_dim : 0);
+    const bool q_in_place = a->q_out == a->q && (a->tokens == 1 || a->q_token == (int64_t)a->n_heads * a->head_dim) && (a->n_heads == 1 || a->q_head == a->head_dim);
+    const bool k_in_place = a->k_out == a->k && (a->tokens == 1 || a->k_token == (int64_t)a->n_kv_heads * a->head_dim) && (a->n_kv_heads == 1 || a->k_head == a->head_dim);
+    HQM_CHECK_ARG((q_in_place || !q_out.meets(q)) && !q_out.meets(k) && !q_out.meets(v), "rope_append_paged: the rotated q shares memory with what is read");
+    HQM_CHECK_ARG(!a->k_out || ((k_in_place || !k_out.meets(k)) && !k_out.meets(q) && !k_out.meets(v) && !k_out.meets(q_out)),
+                  "rope_append_paged: the rotated k shares memory with what is read, or with the rotated q");
+    const Pages pools[2] = {{a->k_pages, a->pages, a->k_page, page_elements}, {a->v_pages, a->pages, a->v_page, page_elements}};
+    HQM_CHECK_ARG(!pools[0].meets(pools[1]), "rope_append_paged: a page of keys shares memory with one of values");
+    for (const Pages& pool : pools)
+        HQM_CHECK_ARG(!pool.meets(q) && !pool.meets(k) && !pool.meets(v) && !pool.meets(q_out) && !pool.meets(k_out),
+                      "rope_append_paged: a page shares memory with what is rotated");
     Append p{(uint16_t*)a->q_out, (uint16_t*)a->k_out, (const uint16_t*)a->q, (const uint16_t*)a->k, (const uint16_t*)a->v, a->q_token, a->q_head, a->k_token,
              a->k_head, a->v_token, a->v_head, (uint16_t*)a->k_pages, (uint16_t*)a->v_pages, a->k_page, a->v_page, a->positions, a->slots,
              (int)a->tokens, a->n_heads, a->n_kv_heads, a->pages, a->page_size, {}};

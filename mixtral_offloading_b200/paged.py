@@ -136,7 +136,9 @@ def rope_append_paged(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, k_pages
     """Rotary embedding of q (T, n_heads, head_dim) and k (T, n_kv_heads, head_dim) at `positions` (T,), and append of k and v
     to the pages at `slots` (T,), in one launch (hqm_rope_append_paged).  Returns the rotated q: `out`, which may be q itself, or
     a new tensor; k_out, which may be k itself, receives the rotated k as well (prompt_attention wants it).  Tokens with a
-    negative slot are left out (their rows of `out` and `k_out` stay as they were; of a new tensor they are not initialised).  No two tokens may have the same slot.  Angles in 64 bits, one rounding."""
+    negative slot are left out (their rows of `out` and `k_out` stay as they were; of a new tensor they are not initialised).
+    No two tokens may have the same slot.
+    Otherwise what is written shares no memory with what is read, nor keys with values (ValueError).  Angles in 64 bits, one rounding."""
     done = _cabi.host().rope_append_paged(q, k, v, k_pages, v_pages, positions, slots, theta, out, k_out)
     if done is not None:
         return done
