@@ -306,6 +306,16 @@ __device__ __forceinline__ float ex2(float x) {
     return r;
 }
 
+// What the weights 2^(x - reference) of a row refer to, from its largest x.  fp16 ends at 2^-24: where the largest weight were 1, a key 17
+// below the largest in e's powers would count in the total and not in the sum with v, 0.4 % of a row with 130000 of them.  So the
+// reference is `lift` lower, the largest weight 2^lift, and maxima, totals and sums of pieces mean that reference.  Not from 2^19 on, where
+// x is known to 2^-5 and worse and the largest weight has to stay clear of 65504.
+constexpr float LIFTED_BELOW = 524288.f;
+template <bool F16>
+__device__ __forceinline__ float reference(float top, float lift) {
+    return F16 && top < LIFTED_BELOW ? top - lift : top;
+}
+
 // Adds the pieces of the units that a cut goes through, of one launch or of two (attn_few.cu).
 int launch_join(const Args& a, const Args* more, int ctas, int D, bool f16, cudaStream_t st);
 // attn_few.cu: up to FEW_TILE rows per key/value head.

@@ -25,6 +25,7 @@ constexpr int THREADS = 32 * (CONSUMERS + 1);
 constexpr int STAGES = 4;
 static_assert(STAGES % 2 == 0, "the halves of the warps take turns: a buffer belongs to one half, or that one would skip every other phase");
 constexpr int UNIT_EXTRA = 1;          // what a unit costs beside its blocks, in blocks
+constexpr float LIFT = 15.f;           // of fp16 weights (attn.cuh): up to 2^15
 
 template <int D>
 struct Shared {
@@ -217,7 +218,7 @@ __device__ __forceinline__ void products(Shared<D>& sh, const Args& a, int cta, 
                 for (int i = 0; i < 2; ++i) {
                     now[i] = fmaxf(now[i], __shfl_xor_sync(0xffffffffu, now[i], 1));
                     now[i] = fmaxf(now[i], __shfl_xor_sync(0xffffffffu, now[i], 2));
-                    now[i] = fmaxf(now[i] * a.scale_log2, top[i]);
+                    now[i] = fmaxf(reference<F16>(now[i] * a.scale_log2, LIFT), top[i]);
                 }
                 if (__any_sync(0xffffffffu, now[0] != top[0] || now[1] != top[1])) {
 #pragma unroll

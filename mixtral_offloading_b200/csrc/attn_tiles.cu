@@ -28,8 +28,8 @@
 // K and V have rings of their own, since warp 8 waits for K only and warp 11 for V only (Ring).
 //
 // The maximum m that a row's weights refer to is raised only when a block exceeds it by more than 2^8: O, which lies in tensor
-// memory, is rescaled a few times per unit instead of once per block, weights grow to 256 at the most, and l and O mean the same
-// whatever m is.
+// memory, is rescaled a few times per unit instead of once per block, weights grow to 256 at the most (of fp16 to 2^15, of which 2^7
+// are there to keep small ones: attn.cuh), and l and O mean the same whatever m is.
 #include <type_traits>
 
 #include "attn_few.cuh"
@@ -47,7 +47,7 @@ typedef Ring<V_RING> VRing;
 constexpr int WEIGHT_WARPS = 8, THREADS = 32 * WEIGHT_WARPS + 128;
 constexpr int REGS_WEIGHTS = 216, REGS_OTHERS = 72;
 static_assert(32 * WEIGHT_WARPS * REGS_WEIGHTS + 128 * REGS_OTHERS <= THREADS * 168, "registers of the launch");
-constexpr float SLACK = 8.f;
+constexpr float SLACK = 8.f, LIFT = 7.f;        // (of fp16 weights: 2^15 together)
 constexpr int UNIT_EXTRA = 2;         // what a unit costs beside its blocks, in blocks
 
 // A part of a unit (Walk), as the warp that walks the list hands it to the others.
@@ -300,9 +300,9 @@ __device__ __forceinline__ void tiles_cta(Shared<D>& sh, const CUtensorMap& qm, 
 #pragma unroll
                     for (int e = 0; e < 4; ++e) top[e] = max3(top[e], __uint_as_float(s[i + 2 * e]), __uint_as_float(s[i + 2 * e + 1]));
                 const float block_top = max2(max3(top[0], top[1], top[2]), top[3]) * a.scale_log2;
-                const bool raise = valid && !(block_top <= m + SLACK);         // (also of NaN)
+                const bool raise = valid && !(block_top <= m + (F16 && m < LIFTED_BELOW ? SLACK + LIFT : SLACK));      // (also of NaN)
                 if (__any_sync(0xffffffffu, raise)) {
-                    float to = max2(m, block_top);
+                    float to = max2(m, reference<F16>(block_top, LIFT));
                     if (to == INFINITY) to = NAN;                              // inf - inf, as the definition has it
                     const float f = to == m ? 1.f : ex2(m - to);
                     m = to;
