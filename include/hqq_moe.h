@@ -375,8 +375,7 @@ typedef struct hqm_paged_append {
     int64_t tokens;
     int32_t n_heads, n_kv_heads, head_dim, pages, page_size;
     int32_t dtype;                      /* 0 bf16, 1 fp16 */
-    float rope_theta;
-    int32_t reserved;
+    float rope_theta, rope_theta_low;   /* theta is their sum: its fp32 value, and what 64 bits have beyond it (or 0) */
 } hqm_paged_append;
 int hqm_rope_append_paged(const hqm_paged_append* a, void* stream);
 

@@ -62,7 +62,7 @@ class HqmPagedAppend(C.Structure):
         ("k_page", C.c_int64), ("v_page", C.c_int64), ("positions", C.c_void_p), ("slots", C.c_void_p),
         ("tokens", C.c_int64), ("n_heads", C.c_int32), ("n_kv_heads", C.c_int32), ("head_dim", C.c_int32),
         ("pages", C.c_int32), ("page_size", C.c_int32), ("dtype", C.c_int32), ("rope_theta", C.c_float),
-        ("reserved", C.c_int32),
+        ("rope_theta_low", C.c_float),
     ]
 
 

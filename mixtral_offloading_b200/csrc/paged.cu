@@ -391,7 +391,8 @@ int hqm_rope_append_paged(const hqm_paged_append* a, void* stream) {
                       a->v_page >= page_elements,
                   "rope_append_paged: %d pages of %d positions (a power of two), %lld and %lld elements apart", a->pages, a->page_size,
                   (long long)a->k_page, (long long)a->v_page);
-    HQM_CHECK_ARG(a->rope_theta > 0.f && isfinite(a->rope_theta), "rope_append_paged: theta %g", (double)a->rope_theta);
+    const double theta = (double)a->rope_theta + (double)a->rope_theta_low;      // (2^-25 of theta turns a position of 10^6 by 10^-3)
+    HQM_CHECK_ARG(theta > 0.0 && isfinite(theta), "rope_append_paged: theta %g", theta);
     if (a->tokens == 0) return HQM_OK;
     HQM_CHECK_ARG(a->q_out && a->q && a->k && a->v && a->k_pages && a->v_pages && a->positions && a->slots, "rope_append_paged: null pointer");
     const int64_t strides = a->q_token | a->q_head | a->k_token | a->k_head | a->v_token | a->v_head | a->k_page | a->v_page;
@@ -415,7 +416,7 @@ int hqm_rope_append_paged(const hqm_paged_append* a, void* stream) {
     Append p{(uint16_t*)a->q_out, (uint16_t*)a->k_out, (const uint16_t*)a->q, (const uint16_t*)a->k, (const uint16_t*)a->v, a->q_token, a->q_head, a->k_token,
              a->k_head, a->v_token, a->v_head, (uint16_t*)a->k_pages, (uint16_t*)a->v_pages, a->k_page, a->v_page, a->positions, a->slots,
              (int)a->tokens, a->n_heads, a->n_kv_heads, a->pages, a->page_size, {}};
-    const double step = pow((double)a->rope_theta, -2.0 / a->head_dim);
+    const double step = pow(theta, -2.0 / a->head_dim);
     double f = 1.0 / (2.0 * 3.14159265358979323846);
     for (int d = 0; d < a->head_dim / 2; ++d, f *= step) p.turns[d] = f;
     const int grid = (int)a->tokens;

@@ -482,13 +482,12 @@ bool result_like(PyObject* obj, const at::Tensor& q, at::Tensor* out) {
     *out = *t;
     return true;
 }
-bool real(PyObject* obj, float* v) {
-    const double d = PyFloat_AsDouble(obj);
-    if (d == -1.0 && PyErr_Occurred()) {
+bool real(PyObject* obj, double* v) {
+    *v = PyFloat_AsDouble(obj);
+    if (*v == -1.0 && PyErr_Occurred()) {
         PyErr_Clear();
         return false;
     }
-    *v = (float)d;
     return true;
 }
 
@@ -504,9 +503,12 @@ PyObject* rope_append_paged(PyObject*, PyObject* const* args, Py_ssize_t n) {
         const at::Tensor *positions = ints(args[5], dev, 1), *slots = ints(args[6], dev, 1);
         const int64_t T = q->size(0);
         hqm_paged_append a = {};
+        double theta;
         if (!k || !v || !positions || !slots || !pool.read(args[3], args[4], *q) || k->sizes() != v->sizes() || k->size(0) != T || k->size(1) != pool.heads ||
-            positions->size(0) != T || slots->size(0) != T || !real(args[7], &a.rope_theta))
+            positions->size(0) != T || slots->size(0) != T || !real(args[7], &theta))
             Py_RETURN_NONE;
+        a.rope_theta = (float)theta;
+        a.rope_theta_low = (float)(theta - a.rope_theta);
         at::AutoDispatchBelowADInplaceOrView guard;
         at::Tensor out;
         if (!result_like(args[8], *q, &out)) Py_RETURN_NONE;
@@ -572,8 +574,9 @@ PyObject* attention(PyObject*, PyObject* const* args, Py_ssize_t n) {
             strides(*v, &c.v_token, &c.v_head);
             c.n_kv_heads = (int32_t)k->size(1);
         }
-        c.scale = 1.f / std::sqrt((float)std::max<int64_t>(q->size(2), 1));
-        if (args[5] != Py_None && !real(args[5], &c.scale)) Py_RETURN_NONE;
+        double scale = 1.f / std::sqrt((float)std::max<int64_t>(q->size(2), 1));
+        if (args[5] != Py_None && !real(args[5], &scale)) Py_RETURN_NONE;
+        c.scale = (float)scale;
         at::AutoDispatchBelowADInplaceOrView guard;
         at::Tensor out;
         if (!result_like(args[6], *q, &out)) Py_RETURN_NONE;

@@ -155,9 +155,10 @@ def rope_append_paged(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, k_pages
     out = _out(q, out)
     if k_out is not None:
         _out(k, k_out, "k_out")
+    high = C.c_float(theta).value
     call = _cabi.HqmPagedAppend(
         out.data_ptr(), None if k_out is None else k_out.data_ptr(), q.data_ptr(), k.data_ptr(), v.data_ptr(), *_strides(q), *_strides(k), *_strides(v), k_pages.data_ptr(),
-        v_pages.data_ptr(), k_page, v_page, positions.data_ptr(), slots.data_ptr(), T, n_heads, n_kv, dim, pages, page_size, code, theta, 0)
+        v_pages.data_ptr(), k_page, v_page, positions.data_ptr(), slots.data_ptr(), T, n_heads, n_kv, dim, pages, page_size, code, high, theta - high)
     with torch.cuda.device(q.device):
         _cabi.check(_cabi.lib().hqm_rope_append_paged(C.byref(call), _cabi.stream_ptr(q.device)))
     return out
