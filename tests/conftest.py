@@ -14,6 +14,17 @@ def pytest_configure(config):
     config.addinivalue_line("markers", "gpu: needs a CUDA device (run on the B200 box)")
 
 
+def pytest_collection_modifyitems(items):
+    """The tests that look at launches through torch's profiler, one file behind the other: it sets its clock against the device's when it is
+    first used, and some 40 seconds later a profile of one launch is empty."""
+    users = ("test_few_row_kernel.py", "test_tma_mode.py")
+    at = [i for i, item in enumerate(items) if item.path.name in users]
+    if at:
+        moved = sorted((items[i] for i in at), key=lambda item: users.index(item.path.name))
+        rest = [item for item in items if item.path.name not in users]
+        items[:] = rest[:at[0]] + moved + rest[at[0]:]
+
+
 @pytest.fixture(scope="session")
 def golden_dir():
     return GOLDEN
