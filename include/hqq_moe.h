@@ -392,7 +392,8 @@ int hqm_rope_append_paged(const hqm_paged_append* a, void* stream);
  *     pages are not used.
  * max_new: no sequence has more new tokens than this (0: nothing is done).  Nothing about lengths is read on the host, so a captured call follows
  * them.  head_dim 64 or 128, scale positive; strides in elements, multiples of 8, rows 16-byte aligned.  scratch: any 16-byte aligned memory
- * of hqm_attention_scratch_bytes bytes that no other call in flight uses (nothing in it has to be initialised). */
+ * of hqm_attention_scratch_bytes bytes that no other call in flight uses (nothing in it has to be initialised); up to 42 MB, two pieces of 256
+ * rows per SM, where a sequence may have more than 16 rows per key/value head. */
 typedef struct hqm_attention {
     void* out;
     const void *q, *k, *v;

@@ -89,7 +89,9 @@ int check(const hqm_attention* c, bool paged, const char* what) {
 
 // Which kernels a call takes: attn_few.cu where its unit holds all new tokens of any sequence, else attn_tiles.cu.  Where the
 // sequences beside the longest have few rows on average, both: those that fit a unit of attn_few.cu run there, at the
-// rate of the memory, and do not fill a tile of 128 rows with four.
+// rate of the memory, and do not fill a tile of 128 rows with four.  30 single tokens and 1, 2, 4, 8 chunks of up to 512, 32 on 8 heads of 128 (in
+// front of every call the caches are overwritten): 85, 89, 103, 145 us by both, 93, 98, 116, 162 by attn_tiles.cu alone.  The rule asks for few
+// rows beside ONE longest sequence, which is what the host knows: of those it takes the first two.
 struct Kernels {
     bool few, tiles;
     static Kernels of(const hqm_attention* c, bool paged) {
@@ -101,7 +103,8 @@ struct Kernels {
 };
 // Whether units are cut.  Where there is a CTA for each and none is long, they are not: the blocks that a CTA then works through one
 // after another cost less than the launch that joins pieces.  What is known here of the lengths are bounds: the table's rows,
-// max_new; the units of a prompt have half as many blocks as the longest on average.  32 on 8 heads of 128, with pieces and
+// max_new (so a table whose rows are far wider than its sequences are long has its units cut); the units of a prompt have half as many
+// blocks as the longest on average.  32 on 8 heads of 128, with pieces and
 // whole: one token on 100 positions 8.6 and 6.6 us, on 300 8.7 and 8.3, on 500 9.0 and 10.5; 60 tokens behind 300 14.3 and 12.6, behind 500
 // 15.2 and 16.3; a prompt of 250 tokens 14.9 and 11.7, of 500 17.4 and 15.0, of 700 20.8 and 18.2.
 bool cuts(const hqm_attention* c, bool paged, int ctas, int per, int block, int most_blocks) {

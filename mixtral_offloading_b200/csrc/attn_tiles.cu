@@ -29,7 +29,8 @@
 //
 // The maximum m that a row's weights refer to is raised only when a block exceeds it by more than 2^8: O, which lies in tensor
 // memory, is rescaled a few times per unit instead of once per block, weights grow to 256 at the most (of fp16 to 2^15, of which 2^7
-// are there to keep small ones: attn.cuh), and l and O mean the same whatever m is.
+// are there to keep small ones: attn.cuh), and l and O mean the same whatever m is.  p is rounded to the type of V, as in attn_few.cuh, with
+// the same errors; l adds it before the rounding.
 #include <type_traits>
 
 #include "attn_few.cuh"
@@ -565,7 +566,8 @@ __global__ void __launch_bounds__(THREADS, 1) attn_tiles_kernel(const __grid_con
 // Single tokens beside chunks: the first CTAs work on the sequences of many rows (a: bound by weights and products), the others on
 // those of few (f: bound by the bytes), at the same time.  How many: so that both take as long, from the lengths; a block of 128
 // positions and 256 rows is taken for MIXED_COST blocks of 64 positions and few rows.  Two chunks of up to 512 tokens among 30 single
-// ones, 32 on 8 heads of 128: 96 us in two launches one after the other; 81, 78, 82 and 96 us with a cost of 2, 3, 4 and 6.
+// ones, 32 on 8 heads of 128: 96 us in two launches one after the other; 81, 78, 82 and 96 us with a cost of 2, 3, 4 and 6.  With 64 columns (in
+// front of every call the caches are overwritten) 79, 68, 71 and 73 us, for one chunk 77, 66, 65 and 68: the same price for both.
 constexpr int MIXED_COST = 3;
 
 template <int D, bool F16>

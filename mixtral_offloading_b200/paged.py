@@ -178,7 +178,7 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     b's rows are cu_seqlens[b] .. cu_seqlens[b + 1] - 1, and its kv_lens[b] positions, the new tokens' last among them, are in the
     pages already.  New token i of n sees positions 0 .. kv_lens[b] - n + i; a row that sees nothing is 0.  max_new: no sequence
     has more new tokens (1 for a decoding step).  scale: 1 / sqrt(head_dim) unless given.  Rows behind the last sequence are
-    left as they were in `out` (of a new tensor they are not initialised), which has to have memory of its own."""
+    left as they were in `out` (of a new tensor they are not initialised), which shares no memory with q or the pages."""
     done = _cabi.host().attention(q, k_pages, v_pages, cu_seqlens, max_new, scale, out, block_table, kv_lens)
     if done is not None:
         return done
